@@ -1,0 +1,370 @@
+"""Performance cases of the 4-bit operators beside the requantised weights.
+
+The optimizer leaves a model's weights in NVFP4: E2M1 codes, an E4M3 scale for 16 values, an FP32 scale on top.  These are the
+calls of a program that computes with such weights: the linear layer (its activations quantised, the product in 4 bits), its two
+gradients (both gradients' operands quantised along the other axis), the quantisation of a tensor by rows or by columns and its
+reading back, and a paged cache of keys and values that is quantised as it is written and read back in 16 bits.  Sizes are those
+of the GPT-2 configurations in bench.py; `draw` gives others of the same ranges.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+own = False
+DEVICE = "cuda"
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+SIZES = {"bf16": 2, "f16": 2, "f32": 4}
+GRID = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)          # E2M1 values of the codes 0 .. 7; code 8 is the sign
+
+
+# ---- the cases ------------------------------------------------------------------------------------------------------------------
+def _linear(name, tokens, inputs, outputs, dtype="bf16", out="bf16", bias=True):
+    return {"name": name, "op": "linear", "tokens": tokens, "inputs": inputs, "outputs": outputs, "dtype": dtype, "out": out, "bias": bias}
+
+
+def _gradients(name, tokens, inputs, outputs, dtype="bf16"):
+    return {"name": name, "op": "gradients", "tokens": tokens, "inputs": inputs, "outputs": outputs, "dtype": dtype}
+
+
+def _round(name, rows, cols, along, dtype):
+    return {"name": name, "op": "requantise", "rows": rows, "cols": cols, "along": along, "dtype": dtype}
+
+
+def _cache(name, sequences, longest, heads, dim, page, new, dtype="bf16"):
+    return {"name": name, "op": "cache", "sequences": sequences, "longest": longest, "heads": heads, "dim": dim, "page": page,
+            "new": new, "dtype": dtype}
+
+
+def listed():
+    return [
+        # One token through the fused query, key and value projection of GPT-2 XL: a step of generation for a single user.
+        _linear("linear, 1 x 1600 -> 4800", 1, 1600, 4800),
+        # A small batch of users in the second MLP projection, a long sum into few outputs; F16 activations.
+        _linear("linear, 24 x 6400 -> 1600", 24, 6400, 1600, dtype="f16", out="f16"),
+        # A prompt of an odd length through the first projection of GPT-2 small.
+        _linear("linear, 1000 x 768 -> 2304", 1000, 768, 2304, bias=False),
+        # A training batch of 16 sequences through the first MLP projection of GPT-2 XL.
+        _linear("linear, 16384 x 1600 -> 6400", 16384, 1600, 6400),
+        # The logits of two sequences over the unpadded vocabulary: rows that start on no boundary, FP32 for the loss.
+        _linear("logits, 2048 x 1600 -> 50257", 2048, 1600, 50257, out="f32", bias=False),
+        # Both gradients of the first MLP projection of GPT-2 medium for eight sequences.
+        _gradients("gradients, 8192 x 1024 -> 4096", 8192, 1024, 4096),
+        # The same of a square projection of GPT-2 XL for one odd prompt: sums over 777 tokens.
+        _gradients("gradients, 777 x 1600 -> 1600", 777, 1600, 1600),
+        # A few FP32 rows of a length that is no multiple of a block, rounded to 4 bits and read back: a calibration's call.
+        _round("requantise, 33 x 1000 by rows", 33, 1000, "rows", "f32"),
+        # A batch's activations quantised along the tokens, as a weight gradient needs them, and read back.
+        _round("requantise, 16384 x 1600 by columns", 16384, 1600, "columns", "bf16"),
+        # One new token for each of 32 users of GPT-2 XL, then everything that they have said so far.
+        _cache("cache, 32 users x 1 token", 32, 1024, 25, 64, 16, "one"),
+        # Whole prompts of GPT-2 medium written to the cache and read back for attention.
+        _cache("cache, 64 prompts", 64, 1024, 16, 64, 64, "all"),
+    ]
+
+
+def _log_int(rng, lo, hi, step=1):
+    """A multiple of `step` in [lo, hi], spread over its logarithm."""
+    v = math.exp(rng.uniform(math.log(lo), math.log(hi + step)))
+    return max(lo, min(hi, int(v) // step * step))
+
+
+def draw(rng):
+    op = rng.choice(["linear", "linear", "gradients", "requantise", "cache"])
+    dtype = rng.choice(["bf16", "bf16", "f16"])
+    if op == "linear":
+        inputs, outputs = _log_int(rng, 768, 6400, 32), _log_int(rng, 768, 50257)
+        tokens = _log_int(rng, 1, min(16384, int(1.6e11 / (inputs * outputs))))
+        return _linear("", tokens, inputs, outputs, dtype, rng.choice([dtype, dtype, "f32"]), rng.random() < 0.5)
+    if op == "gradients":
+        inputs, outputs = _log_int(rng, 256, 6400, 32), _log_int(rng, 256, 6400, 32)
+        return _gradients("", _log_int(rng, 16, min(16384, int(0.8e11 / (inputs * outputs)))), inputs, outputs, dtype)
+    if op == "requantise":
+        cols = _log_int(rng, 48, 6400)
+        return _round("", _log_int(rng, 1, min(32768, 26_000_000 // cols)), cols, rng.choice(["rows", "columns"]), rng.choice([dtype, "f32"]))
+    heads, dim = rng.choice([4, 8, 12, 16, 25]), rng.choice([64, 64, 96, 128])
+    longest = _log_int(rng, 16, 4096)
+    return _cache("", _log_int(rng, 1, max(1, min(64, 60_000_000 // (longest * heads * dim)))), longest, heads, dim, rng.choice([16, 32, 64]),
+                  rng.choice(["one", "all"]), dtype)
+
+
+def work(case):
+    size = SIZES[case["dtype"]]
+    if case["op"] == "linear":
+        m, k, n = case["tokens"], case["inputs"], case["outputs"]
+        return {"bytes": m * k * size + n * k * 9 // 16 + m * n * SIZES[case["out"]] + (4 * n if case["bias"] else 0), "flops": 2 * m * n * k}
+    if case["op"] == "gradients":
+        m, k, n = case["tokens"], case["inputs"], case["outputs"]
+        return {"bytes": m * (k + n) * size + n * k * 9 // 16 + m * k * size + n * k * 4, "flops": 4 * m * n * k}
+    if case["op"] == "requantise":
+        n = case["rows"] * case["cols"]
+        return {"bytes": 2 * n * size, "flops": n}
+    # on average half of the longest sequence is there; keys and values
+    values = 2 * case["sequences"] * case["longest"] // 2 * case["heads"] * case["dim"]
+    new = values if case["new"] == "all" else 2 * case["sequences"] * case["heads"] * case["dim"]
+    return {"bytes": new * size + new * 37 // 64 + values * 37 // 64 + values * size, "flops": values}
+
+
+# ---- inputs: made from the seed alone ----------------------------------------------------------------------------------------------
+def _generator(seed):
+    return torch.Generator(device=DEVICE).manual_seed(seed)
+
+
+def _normal(g, shape, std, outliers=0.0):
+    """Normal values; a share of the columns is 20 times as large, as some channels of a transformer's activations are."""
+    x = torch.randn(shape, device=DEVICE, generator=g) * std
+    if outliers:
+        x *= 1.0 + 19.0 * (torch.rand(shape[-1], device=DEVICE, generator=g) < outliers)
+    return x
+
+
+def _weights(g, rows, k):
+    """A weight matrix as the optimizer leaves it: codes (one a byte), block scales (E4M3 bytes), and the tensor scale max / 1536."""
+    w = torch.randn(rows, k, device=DEVICE, generator=g) * 0.02
+    scale = (w.abs().max() / 1536.0).reshape(1)
+    blocks = w.view(rows, k // 16, 16)
+    s = (blocks.abs().amax(-1) / (6.0 * scale)).to(torch.float8_e4m3fn)
+    codes = _codes(blocks / (s.float() * scale)[..., None]).view(rows, k)
+    return codes, s.view(torch.uint8), scale
+
+
+def _tiled(scales):
+    """Block scales [rows, blocks] in the operand layout of the tensor cores: tiles of 128 rows x 4 blocks, zeros behind the ends."""
+    rows, blocks = scales.shape
+    r, b = -(-rows // 128), -(-blocks // 4)
+    full = torch.zeros(r * 128, b * 4, dtype=torch.uint8, device=DEVICE)
+    full[:rows, :blocks] = scales
+    return full.view(r, 4, 32, b, 4).permute(0, 3, 2, 1, 4).contiguous().view(-1)
+
+
+def _inputs(case, seed):
+    g = _generator(seed)
+    if case["op"] == "linear":
+        m, k, n = case["tokens"], case["inputs"], case["outputs"]
+        x = _normal(g, (m, k), 1.0, 0.002).to(TYPES[case["dtype"]])
+        return {"x": x, "w": _weights(g, n, k), "bias": _normal(g, (n,), 0.1) if case["bias"] else None}
+    if case["op"] == "gradients":
+        m, k, n = case["tokens"], case["inputs"], case["outputs"]
+        x = _normal(g, (m, k), 1.0, 0.002).to(TYPES[case["dtype"]])
+        # F16 gradients come out of a scaled loss
+        grad = _normal(g, (m, n), 1.0e-4 if case["dtype"] == "bf16" else 0.1, 0.002).to(TYPES[case["dtype"]])
+        return {"x": x, "grad": grad, "wt": _weights(g, k, n)}
+    if case["op"] == "requantise":
+        return {"x": _normal(g, (case["rows"], case["cols"]), 1.0, 0.01).to(TYPES[case["dtype"]])}
+    b, longest, page = case["sequences"], case["longest"], case["page"]
+    per = -(-longest // page)
+    lengths = torch.randint(1, longest + 1, (b,), device=DEVICE, generator=g)
+    table = torch.randperm(b * per, device=DEVICE, generator=g).view(b, per)
+    position = torch.arange(longest, device=DEVICE)
+    there = position < lengths[:, None]
+    slot = table.gather(1, (position // page).expand(b, longest)) * page + position % page
+    fresh = there if case["new"] == "all" else position == lengths[:, None] - 1
+    shape = (int(fresh.sum()), case["heads"], case["dim"])
+    old = (b * per * page, case["heads"], case["dim"])
+    return {"lengths": lengths.int(), "table": table.int(), "slots": slot[fresh], "there": there, "slot": slot,
+            "key": _normal(g, shape, 1.0, 0.02).to(TYPES[case["dtype"]]), "value": _normal(g, shape, 0.5).to(TYPES[case["dtype"]]),
+            "old": (_normal(g, old, 1.0, 0.02), _normal(g, old, 0.5))}
+
+
+def prepare(case, seed):
+    """What a program has in hand: the tensors, the weights as operands, the outputs' memory, and with the kernels their handles."""
+    state = {"case": case, **_inputs(case, seed)}
+    like = dict(dtype=TYPES[case["dtype"]], device=DEVICE)
+    if case["op"] == "linear":
+        m, k, n = case["tokens"], case["inputs"], case["outputs"]
+        state["out"] = torch.empty(m, n, dtype=TYPES[case["out"]], device=DEVICE)
+    elif case["op"] == "gradients":
+        m, k, n = case["tokens"], case["inputs"], case["outputs"]
+        state["grad_x"], state["grad_w"] = torch.empty(m, k, **like), torch.empty(n, k, device=DEVICE)
+    elif case["op"] == "requantise":
+        shape = (case["rows"], case["cols"])
+        state["out"] = torch.empty(shape if case["along"] == "rows" else shape[::-1], **like)
+    else:
+        kept = [_pack_cache(x) for x in state.pop("old")]
+        state["cache"] = [[t.view(-1, case["page"], *t.shape[1:]) for t in x] for x in kept]
+        shape = (case["sequences"], case["longest"], case["heads"], case["dim"])
+        state["out"] = [torch.zeros(shape, **like), torch.zeros(shape, **like)]
+    if own:
+        import llmini_b200 as b2
+
+        state["module"] = b2.Nvfp4LinearModule()
+        if case["op"] == "linear":
+            state["weight"] = _operand(b2, *state["w"])
+            state["scratch"] = b2.Nvfp4LinearScratch(m, k, n)
+        elif case["op"] == "gradients":
+            state["weight_t"] = _operand(b2, *state["wt"])
+            state["scratch"] = b2.Nvfp4LinearScratch(m, k, n, backward=True)
+        elif case["op"] == "requantise":
+            rows = case["along"] == "rows"
+            state["operand"] = b2.Nvfp4Operand.empty(*state["out"].shape, per_row=rows)
+            state["amax"] = torch.empty(1, device=DEVICE)
+        else:
+            state["paged"] = b2.Nvfp4PagedCache(*state["cache"])
+    return state
+
+
+def _operand(b2, codes, scales, scale):
+    rows, k = codes.shape
+    packed = codes[:, 0::2] | (codes[:, 1::2] << 4)
+    return b2.Nvfp4Operand(packed.contiguous(), _tiled(scales), scale, rows, k)
+
+
+# ---- plain forms ----------------------------------------------------------------------------------------------------------------
+def _codes(q):
+    """Nearest E2M1 codes (one a byte) of `q`; between two values the even code, beyond 6 the code of 6."""
+    a = q.abs()
+    c = (a > 0.25).byte() + (a >= 0.75).byte() + (a > 1.25).byte() + (a >= 1.75).byte() + (a > 2.5).byte() + (a >= 3.5).byte() + (a > 5.0).byte()
+    return c + 8 * (q < 0).byte()
+
+
+def _power(amax):
+    """The scale of a vector with this maximum: the power of two 2^-10 below it; 1 where nothing is left of the vector."""
+    scale = torch.ldexp(torch.ones_like(amax), torch.frexp(amax)[1] - 11)
+    return torch.where(amax >= 2.0 ** -100, scale, torch.ones_like(scale))
+
+
+def _quantise(x, scale):
+    """Codes and E4M3 scales of blocks of 16 along the last axis, for a `scale` that broadcasts against it."""
+    pad = -x.shape[-1] % 16
+    blocks = torch.nn.functional.pad(x.float(), (0, pad)).unflatten(-1, (-1, 16))
+    s = (blocks.abs().amax(-1) / 6.0 / scale).to(torch.float8_e4m3fn)
+    step = (s.float() * scale)[..., None]
+    q = torch.where(step > 0, blocks / torch.where(step > 0, step, torch.ones_like(step)), torch.zeros_like(blocks))
+    return _codes(q).flatten(-2), s
+
+
+def _values(codes, s, scale):
+    """The values that codes, E4M3 scales and the scale on top stand for, in FP32."""
+    grid = torch.tensor(GRID + tuple(-v for v in GRID), device=DEVICE)
+    v = grid[codes.long()].unflatten(-1, (-1, 16)) * s.view(torch.float8_e4m3fn).float()[..., None]
+    return v.flatten(-2) * scale
+
+
+def _rounded(x, whole=False):
+    """`x` quantised along its last axis and read back: with a scale for each row, or one for the tensor."""
+    a = x.abs().amax().float().expand(x.shape[0], 1) if whole else x.abs().amax(-1, keepdim=True).float()
+    scale = _power(a)
+    return _values(*_quantise(x, scale), scale)[:, : x.shape[-1]]
+
+
+def _pack_cache(x):
+    """Vectors [.., dim] as the cache holds them: packed codes, block scales, and the exponent of the scale on top (E8M0)."""
+    scale = _power(x.abs().amax(-1, keepdim=True).float())
+    codes, s = _quantise(x, scale)
+    return codes[..., 0::2] | (codes[..., 1::2] << 4), s.view(torch.uint8), (torch.frexp(scale[..., 0])[1] + 126).to(torch.uint8)
+
+
+def _unpack_cache(packed, s, exponent):
+    codes = torch.stack([packed & 15, packed >> 4], -1).flatten(-2)
+    return _values(codes, s, torch.ldexp(torch.ones(exponent.shape, device=DEVICE), exponent.int() - 127)[..., None])
+
+
+def _plain_linear(state):
+    y = _rounded(state["x"]) @ _values(*state["w"]).T
+    if state["bias"] is not None:
+        y += state["bias"]
+    return y.to(state["out"].dtype)
+
+
+def _plain_gradients(state):
+    grad, x = state["grad"], state["x"]
+    grad_x = _rounded(grad) @ _values(*state["wt"]).T
+    grad_w = _rounded(grad.T, whole=True) @ _rounded(x.T, whole=True).T
+    return grad_x.to(grad.dtype), grad_w
+
+
+def _plain_requantise(state):
+    x = state["x"]
+    return (_rounded(x) if state["case"]["along"] == "rows" else _rounded(x.T, whole=True)).to(x.dtype)
+
+
+def _plain_side(state, which, new):
+    """One of keys and values: the new vectors written to their slots, then every sequence read back."""
+    kept, out = state["cache"][which], state["out"][which]
+    flat = [t.view(-1, *t.shape[2:]) for t in kept]
+    packed = _pack_cache(new)
+    flat[0][state["slots"]] = packed[0]
+    flat[1][state["slots"]] = packed[1]
+    flat[2][state["slots"]] = packed[2]
+    at = state["slot"][state["there"]]
+    out[state["there"]] = _unpack_cache(flat[0][at], flat[1][at], flat[2][at]).to(out.dtype)
+    return out
+
+
+def run(state):
+    op = state["case"]["op"]
+    if not own:
+        if op == "linear":
+            return _plain_linear(state)
+        if op == "gradients":
+            return _plain_gradients(state)
+        if op == "requantise":
+            return _plain_requantise(state)
+        return _plain_side(state, 0, state["key"]), _plain_side(state, 1, state["value"])
+    m = state["module"]
+    if op == "linear":
+        m.linear_forward(state["x"], state["weight"], state["out"], state["scratch"], bias=state["bias"])
+        return state["out"]
+    if op == "gradients":
+        m.linear_backward(state["grad"], state["x"], state["weight_t"], state["grad_x"], state["grad_w"], state["scratch"])
+        return state["grad_x"], state["grad_w"]
+    if op == "requantise":
+        if state["case"]["along"] == "rows":
+            m.quantize_rows(state["x"], state["operand"])
+        else:
+            m.quantize_columns(state["x"], state["operand"], state["amax"])
+        m.decode(state["operand"], state["out"])
+        return state["out"]
+    m.cache_write(state["paged"], state["slots"], state["key"], state["value"])
+    m.cache_read(state["paged"], state["table"], state["lengths"], *state["out"])
+    return tuple(state["out"])
+
+
+# ---- in 64 bits, from the definition ------------------------------------------------------------------------------------------------
+def _exact_round(x, amax):
+    """Rows of `x` as 4-bit values, in FP64: the scale 2^(floor(log2 amax) - 10), block scales on the E4M3 grid nearest to max / 6,
+    values on the E2M1 grid nearest to the quotient; the even neighbour between two."""
+    x, amax = x.double(), amax.double()
+    top = torch.where(amax >= 2.0 ** -100, torch.exp2(torch.floor(torch.log2(amax.clamp(min=2.0 ** -100))) - 10), torch.ones_like(amax))
+    cols = x.shape[-1]
+    wide = torch.zeros(*x.shape[:-1], -(-cols // 16) * 16, dtype=torch.float64, device=DEVICE)
+    wide[..., :cols] = x
+    b = wide.view(*x.shape[:-1], -1, 16)
+    t = b.abs().amax(-1) / 6 / top[..., None]
+    ulp = torch.exp2(torch.floor(torch.log2(t.clamp(min=2.0 ** -6))) - 3)          # E4M3: 3 bits, subnormal below 2^-6
+    step = (torch.round(t / ulp) * ulp * top[..., None])[..., None]
+    q = torch.where(step > 0, b / step.clamp(min=1e-300), 0.0)
+    unit = torch.exp2(torch.floor(torch.log2(q.abs().clamp(min=1.0, max=6.0))) - 1)  # E2M1: 1 bit, subnormal below 1
+    r = (torch.round(q / unit) * unit).clamp(-6, 6)
+    return (r * step).view(wide.shape)[..., :cols]
+
+
+def _exact_weights(codes, s, scale):
+    mantissa, exponent = (codes & 1).double(), (codes >> 1 & 3).double()
+    v = torch.where(exponent > 0, (1 + mantissa / 2) * torch.exp2(exponent - 1), mantissa / 2) * torch.where(codes >= 8, -1.0, 1.0)
+    e, f = (s >> 3 & 15).double(), (s & 7).double()
+    w = torch.where(e > 0, (1 + f / 8) * torch.exp2(e - 7), f * 2.0 ** -9)
+    return (v.view(*w.shape, 16) * w[..., None]).flatten(-2) * scale.double()
+
+
+def exact(case, seed):
+    given = _inputs(case, seed)
+    if case["op"] == "linear":
+        x = given["x"]
+        y = _exact_round(x, x.abs().amax(-1)) @ _exact_weights(*given["w"]).T
+        return y if given["bias"] is None else y + given["bias"].double()
+    if case["op"] == "gradients":
+        x, grad = given["x"], given["grad"]
+        grad_x = _exact_round(grad, grad.abs().amax(-1)) @ _exact_weights(*given["wt"]).T
+        whole = lambda t: _exact_round(t.T, t.abs().amax().expand(t.shape[1]))
+        return grad_x, whole(grad) @ whole(x).T
+    if case["op"] == "requantise":
+        x = given["x"]
+        return _exact_round(x, x.abs().amax(-1)) if case["along"] == "rows" else _exact_round(x.T, x.abs().amax().expand(x.shape[1]))
+    both = []
+    for old, new in zip(given["old"], (given["key"], given["value"])):
+        kept = _exact_round(old, old.abs().amax(-1))
+        kept[given["slots"]] = _exact_round(new, new.abs().amax(-1))
+        both.append(torch.where(given["there"][..., None, None], kept[given["slot"]], 0.0))
+    return tuple(both)

@@ -61,15 +61,13 @@
 
 #include "common.cuh"
 #include "internal.h"
+#include "sm100.cuh"
 
 namespace b2 {
 
 namespace {
 
 constexpr int kBoxBytes = 64 * 128;          // 64 rows x 128 bytes
-constexpr int kSmemLimit = 227 * 1024;
-constexpr uint32_t kSpinLimit = 1u << 24;    // hard cap on polls, whatever the timer says
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 // TM x BN is the tile of a CTA, or of a pair of CTAs; a pair's CTAs hold half of its rows of A and half of its rows of B each.
 template <int TM, int BN, bool PAIR, bool CHAINED>
@@ -100,87 +98,6 @@ struct Cfg {
     static constexpr int kStages = kMaxStages < 8 ? kMaxStages : 8;
     static constexpr int kSmemBytes = kStages * kStageBytes + kBarrierBytes + 1024;
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-// shared::cluster address of the same offset in CTA `rank` of this cluster
-__device__ __forceinline__ uint32_t map_to_cta(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_cta_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Arrive on a barrier given by its shared::cluster address (own or peer CTA).  For tensor memory that has been read, whose order
-// tcgen05.fence::before_thread_sync keeps: relaxed, because release semantics at cluster scope would make the thread wait for
-// its stores.
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok;
-}
-// Non-blocking probe of a barrier phase.  (mbarrier.try_wait may suspend the thread for a system-dependent time,
-// measured here at about 5 us, before it reports that the phase is not complete; that is right for a wait, not
-// for a probe.)
-__device__ __forceinline__ uint32_t mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok;
-}
-__device__ __forceinline__ uint64_t global_timer_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// Bounded wait (about two seconds of wall clock).  Returns false when the limit ran out or
-// another role of this CTA already gave up.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
-#pragma unroll 1
-    for (int it = 0; it < 128; ++it)
-        if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t start = global_timer_ns();
-#pragma unroll 1
-    for (uint32_t it = 0; it < kSpinLimit; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        if (global_timer_ns() - start > kWaitLimitNs) break;
-        __nanosleep(it >= 1024 ? 256 : 32);
-    }
-    *abort_flag = 1;
-    return false;
-}
-
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag) {
-    return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity, abort_flag);
-}
 
 __device__ __forceinline__ uint32_t ld_acquire_gpu(const uint32_t *p) {
     uint32_t v;
@@ -255,143 +172,6 @@ __device__ __forceinline__ uint32_t hand_get(volatile uint64_t *ring, uint32_t s
     }
     *abort_flag = 1;
     return kNoTile;
-}
-
-template <bool PAIR>
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, uint64_t map, uint32_t bar, int x, int y) {
-    if (PAIR)
-        asm volatile(
-            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-            : "memory");
-    else
-        asm volatile(
-            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
-            : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, uint64_t map, uint32_t bar, int x, int y, int z) {
-    if (PAIR)
-        asm volatile(
-            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-            : "memory");
-    else
-        asm volatile(
-            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-            ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
-            : "memory");
-}
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// Arrive on `bar` once every MMA issued so far has retired.  PAIR: the arrival is delivered
-// to the barrier at this offset in both CTAs of the pair.
-template <bool PAIR>
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    if (PAIR)
-        asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-            ::"r"(bar), "h"((uint16_t)3)
-            : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                     : "memory");
-}
-template <bool PAIR>
-__device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                       uint32_t accumulate) {
-    if (PAIR)
-        asm volatile(
-            "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
-            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
-            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-            : "memory");
-}
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(r));
-    return r != 0u;
-}
-// 32 lanes x 32 consecutive 32-bit columns: thread i of the warp receives row (lane base + i).
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-// 32 lanes x 16 consecutive 32-bit columns
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-// 16 lanes x 64 consecutive 32-bit columns, in the layout of an MMA accumulator: thread i receives columns 8 j + 2 (i % 4) and
-// the next one of row i / 4 in r[4 j], r[4 j + 1], those of row 8 + i / 4 in r[4 j + 2], r[4 j + 3].
-__device__ __forceinline__ void tc_ld_16x64(uint32_t taddr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-// Four words of each of four neighbouring lanes, transposed: word k of lane s becomes word s of lane k.
-__device__ __forceinline__ void quad_transpose(uint32_t &w0, uint32_t &w1, uint32_t &w2, uint32_t &w3, uint32_t lane) {
-    const bool odd = lane & 1u, high = lane & 2u;
-    const uint32_t p = __shfl_xor_sync(0xffffffffu, odd ? w0 : w1, 1), r = __shfl_xor_sync(0xffffffffu, odd ? w2 : w3, 1);
-    if (odd) { w0 = p; w2 = r; } else { w1 = p; w3 = r; }
-    const uint32_t t = __shfl_xor_sync(0xffffffffu, high ? w0 : w2, 2), u = __shfl_xor_sync(0xffffffffu, high ? w1 : w3, 2);
-    if (high) { w0 = t; w1 = u; } else { w2 = t; w3 = u; }
-}
-// 32 bytes, one sector, to a 32-byte aligned address
-__device__ __forceinline__ void st_global_32(void *p, const uint32_t *v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
-__device__ __forceinline__ void tc_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory matrix descriptor, 128-byte swizzle, descriptor version 1 (sm_100).
-//   K-major operand  (rows = M/N index, 128 bytes of K per row): 8-row groups are 1024 bytes
-//   apart (stride byte offset); the leading byte offset is unused.
-//   MN-major operand (rows = K index, 128 bytes = 64 M/N elements per row): 8-row groups of K
-//   are 1024 bytes apart (stride), 64-element groups of M/N are one 64 x 64 box (8192 bytes)
-//   apart (leading).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-    uint64_t d = 0;
-    d |= (uint64_t)((addr & 0x3ffffu) >> 4);
-    d |= (uint64_t)((lbo_bytes >> 4) & 0x3fffu) << 16;
-    d |= (uint64_t)((sbo_bytes >> 4) & 0x3fffu) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-// Instruction descriptor for kind::f16: FP32 accumulate, A/B format F16 (0) or BF16 (1),
-// per-operand major bit, N >> 3 at bit 17, M >> 4 at bit 24.
-__device__ __forceinline__ uint32_t instr_desc(int m, int n, int f16, uint32_t a_mn, uint32_t b_mn) {
-    uint32_t fmt = f16 ? 0u : 1u;
-    return (1u << 4) | (fmt << 7) | (fmt << 10) | (a_mn << 15) | (b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // What the roles of a CTA need to know about the tile they work on, written by the CTA's scheduler warp into a

@@ -1,0 +1,46 @@
+// Host-side prototypes of the 4-bit operators (fp4_kernels.cu, fp4_gemm_sm100.cu; the entry points are in fp4_api.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/llmini_b200_fp4.h"
+
+namespace b2 {
+
+// Every kernel of these operators waits for the launch in front of it before it touches global memory (griddepcontrol.wait),
+// so all of them are launched with programmatic dependent launch: their prologues run while that one ends.
+template <typename... P, typename... A>
+inline cudaError_t overlapped_launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// ---- fp4_kernels.cu --------------------------------------------------------------------------------------------------
+cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s);
+// Scales on top of parts of x, whose largest is the tensor's: writes `*count` (at most B2_NVFP4_MAXIMA) of them.
+cudaError_t launch_fp4_maxima(const b2_matrix &x, float *maxima, uint32_t *count, int sm_count, cudaStream_t s);
+cudaError_t launch_fp4_quantize_columns(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count,
+                                        int sm_count, cudaStream_t s);
+cudaError_t launch_fp4_decode(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s);
+cudaError_t launch_fp4_cache_write(const b2_nvfp4_cache *caches, const b2_vectors *tokens, uint32_t count, const int64_t *slots,
+                                   uint32_t token_count, cudaStream_t s);
+cudaError_t launch_fp4_cache_read(const b2_nvfp4_cache *caches, const b2_vectors *out, uint32_t count, const int32_t *table,
+                                  uint32_t table_width, const int32_t *lengths, uint32_t sequences, uint32_t max_tokens,
+                                  cudaStream_t s);
+
+// ---- fp4_gemm_sm100.cu -----------------------------------------------------------------------------------------------
+cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias,
+                              bool accumulate, int sm_count, cudaStream_t s);
+cudaError_t fp4_gemm_status(uint32_t *status, cudaStream_t s);
+
+}  // namespace b2

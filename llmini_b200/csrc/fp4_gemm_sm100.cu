@@ -1,0 +1,425 @@
+// C[M][N] = A B^T of two NVFP4 operands on the block-scaled tensor cores of sm_100a: tcgen05.mma kind::mxf4nvf4 with an E4M3
+// scale for 16 values of K, FP32 accumulators in tensor memory, operands and their block scales staged by TMA, the scales copied
+// on from shared to tensor memory by tcgen05.cp in front of the MMAs that read them.
+//
+// The operands' rows are 128-byte swizzled panels as in the Newton-Schulz GEMM (ns_gemm_sm100.cu): 128 bytes are 256 values of K,
+// four MMAs.  The block scales of 128 rows and 64 values of K are a 512-byte tile, stored as the copy wants it.
+#include <algorithm>
+#include <atomic>
+
+#include <cuda.h>
+
+#include "common.cuh"
+#include "fp4.h"
+#include "sm100.cuh"
+
+namespace b2 {
+
+namespace {
+
+constexpr uint32_t kStageK = 256;       // values of K in a pipeline stage
+constexpr uint32_t kScaleTile = 512;    // bytes: 128 rows x 64 values of K
+constexpr uint32_t kScaleBand = kStageK / 64 * kScaleTile;   // a stage's scales of 128 rows
+
+// Set when a bounded wait ran out (b2_nvfp4_status).
+__device__ uint32_t g_fp4_status;
+
+// D (+)= A B^T over 64 values of K; the scales' addresses are columns of tensor memory
+template <bool PAIR>
+__device__ __forceinline__ void tc_mma_fp4(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                           uint32_t accumulate) {
+    if (PAIR)
+        asm volatile(
+            "{ .reg .pred p; setp.ne.b32 p, %6, 0; "
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p; }"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{ .reg .pred p; setp.ne.b32 p, %6, 0; "
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p; }"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+// A 512-byte tile of scales from shared memory to four columns of tensor memory, the same in every lane quarter; PAIR: in both
+// CTAs, each from its own shared memory.
+template <bool PAIR>
+__device__ __forceinline__ void tc_copy_scales(uint32_t tmem, uint64_t desc) {
+    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+}
+// Descriptor of such a tile: no swizzle, 8 rows of 16 bytes after one another.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// Instruction descriptor for kind::mxf4nvf4: A and B E2M1 (1), scales UE4M3 (0), N >> 3 at bit 17, M >> 4 at bit 24.
+__device__ __forceinline__ uint32_t fp4_instr_desc(uint32_t m, uint32_t n) {
+    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+struct Epilogue {
+    uint8_t *c;
+    uint64_t pitch;            // bytes
+    const float *scale_a;      // one, or one a row of A
+    const float *scale_b;
+    const float *bias;         // null or [N]
+    uint32_t M, N;
+    uint32_t a_rows, b_rows;   // a scale for every row of A (B)
+    uint32_t type;             // of c
+    uint32_t accumulate;
+    uint32_t vec;              // rows of c start on 32-byte boundaries
+};
+
+// 32 columns from `col` on of row `row`, `acc` their sums: scaled, biased, rounded, stored.
+__device__ __forceinline__ void store_columns(const Epilogue &e, uint32_t row, uint32_t col, const uint32_t *acc, float sa) {
+    if (row >= e.M || col >= e.N) return;
+    float v[32];
+    const float sb = e.b_rows ? 1.0f : *e.scale_b;
+    const float s = sa * sb;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]) * s;
+    const uint32_t n = min(e.N - col, 32u);
+    if (e.b_rows) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if ((uint32_t)i < n) v[i] *= e.scale_b[col + i];
+    }
+    if (e.bias) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if ((uint32_t)i < n) v[i] += e.bias[col + i];
+    }
+    if (e.type == B2_TYPE_F32) {
+        float *p = reinterpret_cast<float *>(e.c + (uint64_t)row * e.pitch) + col;
+        if (n == 32 && e.vec) {
+            if (e.accumulate) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float4 o = reinterpret_cast<const float4 *>(p)[i];
+                    v[4 * i] += o.x; v[4 * i + 1] += o.y; v[4 * i + 2] += o.z; v[4 * i + 3] += o.w;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st_global_32(p + 8 * i, reinterpret_cast<const uint32_t *>(v) + 8 * i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if ((uint32_t)i < n) p[i] = e.accumulate ? p[i] + v[i] : v[i];
+        }
+    } else {
+        uint32_t w[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = pack_operands(v[2 * i], v[2 * i + 1], e.type == B2_TYPE_F16);
+        uint16_t *p = reinterpret_cast<uint16_t *>(e.c + (uint64_t)row * e.pitch) + col;
+        if (n == 32 && e.vec) {
+            st_global_32(p, w);
+            st_global_32(p + 16, w + 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if ((uint32_t)i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    }
+}
+
+// Tile of a CTA (128 x BN), or of a pair of CTAs (256 x BN): each holds 128 rows of A, half of the rows of B and all of B's scales.
+template <bool PAIR, int BN>
+struct FCfg {
+    static constexpr uint32_t kTileM = PAIR ? 256 : 128;
+    static constexpr uint32_t kBRows = PAIR ? BN / 2 : BN;
+    static constexpr uint32_t kBands = BN / 128;
+    static constexpr uint32_t kABytes = 128 * 128, kBBytes = kBRows * 128;
+    static constexpr uint32_t kSfa = kABytes + kBBytes, kSfb = kSfa + kScaleBand;
+    static constexpr uint32_t kStageBytes = kSfb + kBands * kScaleBand;
+    static_assert(kStageBytes % 1024 == 0 && kSfa % 1024 == 0, "panels start on 1024-byte boundaries");
+    // Tensor memory.  Two accumulators of 256 columns leave no room for scales, so they share 48 columns: the epilogue reads
+    // these first, and the other accumulator's MMAs begin when it has.
+    static constexpr uint32_t kShared = BN == 256 ? 48 : 0;
+    static constexpr uint32_t kAcc1 = BN - kShared;
+    static constexpr uint32_t kSfaCol = 2 * BN - kShared, kSfbCol = kSfaCol + 16;
+    static_assert(kSfbCol + 16 * kBands <= 512, "tensor memory");
+    static constexpr uint32_t kTmemCols = 512;
+    // warps: producers of A, of B and of the scales, the MMA issuer, eight epilogue warps
+    static constexpr int kProducerA = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 8, kProducerB = 10, kProducerS = 11;
+    static constexpr int kThreads = 12 * 32;
+    static constexpr uint32_t kControl = 256;
+    static constexpr uint32_t kMaxStages = ((uint32_t)kSmemLimit - kControl - 1024) / kStageBytes;
+    static constexpr uint32_t kStages = kMaxStages < 6 ? kMaxStages : 6;
+    static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kControl + 1024;
+};
+
+template <bool PAIR, int BN>
+__global__ void __launch_bounds__((FCfg<PAIR, BN>::kThreads), 1)
+k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
+           const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ Epilogue epi, uint32_t K, uint32_t tiles_m, uint32_t tiles) {
+    using C = FCfg<PAIR, BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kStages * C::kStageBytes);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * C::kStages + 4);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    static_assert((2 * C::kStages + 4) * 8 + 8 <= C::kControl, "control region");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
+    const uint32_t first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
+    const uint32_t bar0 = smem_u32(bars), stage0 = smem_u32(smem);
+    auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (C::kStages + s); };
+    auto tfull_bar = [&](uint32_t a) { return bar0 + 8u * (2 * C::kStages + a); };
+    auto tempty_bar = [&](uint32_t a) { return bar0 + 8u * (2 * C::kStages + 2 + a); };
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < C::kStages; ++s) {
+            mbar_init(full_bar(s), 3);   // the leader's three producers
+            mbar_init(empty_bar(s), 1);
+        }
+        for (uint32_t a = 0; a < 2; ++a) {
+            mbar_init(tfull_bar(a), 1);
+            mbar_init(tempty_bar(a), PAIR ? 2 * C::kEpiWarps : C::kEpiWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sa) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sb) : "memory");
+    }
+    if (warp == C::kMmaWarp) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(C::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (PAIR) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    stream_enter();
+
+    const uint32_t stages = (K + kStageK - 1) / kStageK;
+    // rows of B that the MMAs of a tile take: what there is of them, rounded up so that a pair's halves are whole 8-row groups
+    auto mma_n = [&](uint32_t tile_n) { return min((uint32_t)BN, (epi.N - tile_n * BN + 31u) / 32u * 32u); };
+
+    if (warp == C::kProducerA || warp == C::kProducerB || warp == C::kProducerS) {
+        if (lane == 0) {
+            const uint32_t leader_full = PAIR ? map_to_cta(full_bar(0), 0) : full_bar(0);
+            const uint32_t bytes = (warp == C::kProducerA ? C::kABytes : warp == C::kProducerB ? C::kBBytes : (1 + C::kBands) * kScaleBand) * (PAIR ? 2u : 1u);
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            for (uint32_t t = first; ok && t < tiles; t += stride) {
+                const uint32_t tile_m = t % tiles_m, tile_n = t / tiles_m;
+                for (uint32_t kb = 0; kb < stages; ++kb) {
+                    if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) { ok = false; break; }
+                    if (rank == 0) mbar_expect_tx(full_bar(stage), bytes);
+                    const uint32_t dst = stage0 + stage * C::kStageBytes, fb = leader_full + 8u * stage;
+                    if (warp == C::kProducerA)
+                        tma_load_2d<PAIR>(dst, reinterpret_cast<uint64_t>(&map_a), fb, (int)(kb * 128), (int)(tile_m * C::kTileM + rank * 128));
+                    else if (warp == C::kProducerB)
+                        tma_load_2d<PAIR>(dst + C::kABytes, reinterpret_cast<uint64_t>(&map_b), fb, (int)(kb * 128),
+                                          (int)(tile_n * BN + (PAIR ? rank * (mma_n(tile_n) / 2) : 0u)));
+                    else {
+                        tma_load_2d<PAIR>(dst + C::kSfa, reinterpret_cast<uint64_t>(&map_sa), fb, (int)(kb * (kScaleBand / 8)),
+                                          (int)(tile_m * (C::kTileM / 128) + rank));
+                        tma_load_2d<PAIR>(dst + C::kSfb, reinterpret_cast<uint64_t>(&map_sb), fb, (int)(kb * (kScaleBand / 8)), (int)(tile_n * C::kBands));
+                    }
+                    if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == C::kMmaWarp) {
+        if (rank == 0) {
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const uint64_t desc0 = smem_desc(__shfl_sync(0xffffffffu, stage0, 0), 0, 1024);
+            const uint64_t sdesc0 = scale_desc(__shfl_sync(0xffffffffu, stage0, 0));
+            uint32_t stage = 0, phase = 0, it = 0;
+            bool ok = true;
+            for (uint32_t t = first; ok && t < tiles; t += stride, ++it) {
+                const uint32_t idesc = fp4_instr_desc(C::kTileM, mma_n(t / tiles_m));
+                // the accumulator is free: its last tile has been read, and, where the two share columns, the other one's these
+                if (C::kShared ? it >= 1 : it >= 2) {
+                    const uint32_t prev = C::kShared ? it - 1 : it - 2;
+                    if (!__all_sync(0xffffffffu, mbar_wait(tempty_bar(prev & 1u), (prev >> 1) & 1u, abort_flag))) break;
+                }
+                tc_fence_after();
+                const uint32_t d_tmem = tmem + (it & 1u) * C::kAcc1;
+                for (uint32_t kb = 0; kb < stages; ++kb) {
+                    if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag))) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t ad = desc0 + stage * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
+                    const uint64_t sd = sdesc0 + ((stage * C::kStageBytes + C::kSfa) >> 4);
+                    if (elect_one()) {
+                        const uint32_t steps = min(4u, (K - kb * kStageK + 63u) / 64u);
+                        for (uint32_t j = 0; j < steps; ++j) {
+                            tc_copy_scales<PAIR>(tmem + C::kSfaCol + 4 * j, sd + j * (kScaleTile >> 4));
+#pragma unroll
+                            for (uint32_t b = 0; b < C::kBands; ++b)
+                                tc_copy_scales<PAIR>(tmem + C::kSfbCol + 4 * (j * C::kBands + b), sd + (((1 + b) * kScaleBand + j * kScaleTile) >> 4));
+                        }
+                        for (uint32_t j = 0; j < steps; ++j)
+                            tc_mma_fp4<PAIR>(d_tmem, ad + 2 * j, bd + 2 * j, idesc, tmem + C::kSfaCol + 4 * j, tmem + C::kSfbCol + 4 * j * C::kBands,
+                                             kb != 0 || j != 0 ? 1u : 0u);
+                        tc_commit<PAIR>(empty_bar(stage));
+                        if (kb + 1 == stages) tc_commit<PAIR>(tfull_bar(it & 1u));
+                    }
+                    __syncwarp();
+                    if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+        }
+    } else {
+        // Warp w reads tensor-memory lanes 32 (w % 4) .. +31, and every other unit of 32 columns.
+        const uint32_t q = warp & 3, half = (warp - C::kEpiWarp0) >> 2;
+        const uint32_t tempty_leader = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
+        constexpr uint32_t kUnits = BN / 32;
+        uint32_t it = 0;
+        for (uint32_t t = first; t < tiles; t += stride, ++it) {
+            const uint32_t tile_m = t % tiles_m, tile_n = t / tiles_m;
+            const uint32_t row = tile_m * C::kTileM + rank * 128 + 32 * q + lane;
+            const float sa = row < epi.M ? epi.scale_a[epi.a_rows ? row : 0] : 0.0f;
+            const uint32_t n = mma_n(tile_n);
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(it & 1u), (it >> 1) & 1u, abort_flag))) break;
+            tc_fence_after();
+            const uint32_t acc = tmem_base + (it & 1u) * C::kAcc1 + ((32u * q) << 16);
+#pragma unroll 1
+            for (uint32_t i = 0; i < kUnits / 2; ++i) {
+                // where the accumulators share columns, these first: the last ones of the first, the first ones of the second
+                const uint32_t p = 2 * i + half, unit = C::kShared && (it & 1u) == 0 ? kUnits - 1 - p : p;
+                uint32_t r[32];
+                const bool there = unit * 32 < n;
+                if (there) {
+                    tc_ld32(acc + unit * 32, r);
+                    tc_ld_wait();
+                }
+                if (i == (C::kShared ? 0 : kUnits / 2 - 1)) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * (it & 1u));
+                }
+                if (there) store_columns(epi, row, tile_n * BN + unit * 32, r, sa);
+            }
+        }
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 4096; ++i) __nanosleep(512);   // what is in flight lands
+        if (threadIdx.x == 0) atomicExch(&g_fp4_status, 1u);
+        __syncthreads();
+    }
+    if (PAIR) cluster_sync_all();
+    if (warp == C::kMmaWarp) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::kTmemCols) : "memory");
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                   CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled() {
+    static const EncodeTiledFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+// Codes: rows of cols / 2 bytes (bytes behind them read as zero), boxes of 128 bytes x box_rows, 128-byte swizzle.
+bool codes_map(CUtensorMap *m, const b2_nvfp4_operand &o, uint32_t box_rows) {
+    const EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {o.cols / 2, o.rows}, strides[1] = {o.row_bytes};
+    const cuuint32_t box[2] = {128, box_rows}, step[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, o.bytes, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Scales: a row of 8-byte words for every band of 128 rows, boxes of a stage's worth x box_bands.
+bool scales_map(CUtensorMap *m, const b2_nvfp4_operand &o, uint32_t box_bands) {
+    const EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const uint64_t tiles = (o.cols / 16 + 3) / 4;
+    const cuuint64_t dims[2] = {tiles * (kScaleTile / 8), ((uint64_t)o.rows + 127) / 128}, strides[1] = {tiles * kScaleTile};
+    const cuuint32_t box[2] = {kScaleBand / 8, box_bands}, step[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, o.scales, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Raises a kernel's limit of shared memory on the current device, once; `done`: the devices on which it has been.
+template <typename K>
+cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1u)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+}
+
+template <bool PAIR, int BN>
+cudaError_t gemm_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const Epilogue &epi, int sm_count, cudaStream_t s) {
+    using C = FCfg<PAIR, BN>;
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(k_fp4_gemm<PAIR, BN>, C::kSmemBytes, done);
+    if (e != cudaSuccess) return e;
+    CUtensorMap map_a, map_b, map_sa, map_sb;
+    if (!codes_map(&map_a, a, 128) || !codes_map(&map_b, b, C::kBRows) || !scales_map(&map_sa, a, 1) || !scales_map(&map_sb, b, C::kBands))
+        return cudaErrorInvalidValue;
+    const uint32_t tiles_m = (a.rows + C::kTileM - 1) / C::kTileM, tiles_n = (b.rows + BN - 1) / BN;
+    const uint64_t tiles = (uint64_t)tiles_m * tiles_n;
+    if (tiles > 0x7fffffffu) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 2 : 1;
+    const uint32_t groups = (uint32_t)std::min<uint64_t>(tiles, PAIR ? sm_count / 2 : sm_count);
+    cfg.gridDim = dim3(PAIR ? 2 * groups : groups);
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<PAIR, BN>, map_a, map_b, map_sa, map_sb, epi, a.cols, tiles_m, (uint32_t)tiles);
+}
+
+}  // namespace
+
+cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias, bool accumulate,
+                              int sm_count, cudaStream_t s) {
+    const uint64_t size = c.type == B2_TYPE_F32 ? 4 : 2;
+    Epilogue epi = {};
+    epi.c = static_cast<uint8_t *>(c.data);
+    epi.pitch = c.ld * size;
+    epi.scale_a = a.scale;
+    epi.scale_b = b.scale;
+    epi.bias = bias;
+    epi.M = a.rows;
+    epi.N = b.rows;
+    epi.a_rows = a.scale_count != 1;
+    epi.b_rows = b.scale_count != 1;
+    epi.type = c.type;
+    epi.accumulate = accumulate;
+    epi.vec = reinterpret_cast<uintptr_t>(c.data) % 32 == 0 && epi.pitch % 32 == 0;
+    return gemm_impl<false, 128>(a, b, epi, sm_count, s);
+}
+
+cudaError_t fp4_gemm_status(uint32_t *status, cudaStream_t s) {
+    uint32_t *word = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(reinterpret_cast<void **>(&word), g_fp4_status);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(status, word, sizeof *status, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaMemsetAsync(word, 0, sizeof *word, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    return e;
+}
+
+}  // namespace b2

@@ -1,0 +1,584 @@
+// Quantisation of activations and gradients to NVFP4 by rows and by columns, reading 4-bit tensors back, and the paged cache.
+// All of it streams: what bounds these kernels is the way to memory and back.
+//
+// The arithmetic, and why it is exact.  With g = 2^e every decision of the quantiser compares a value with a number of few bits.
+//   Block scale: t = RN(b / 6) for b = amax of the block / g, s = e4m3(t).  A border of the E4M3 grid has 5 bits; if b / 6 is no
+//   border, b differs from 6 borders' product by at least an ulp of b, more than half an ulp of the border: RN(b / 6) is on the
+//   right side of it, and it is the border exactly where b / 6 is.
+//   Code: q = x / g / s.  A border of the E2M1 grid times s has at most 7 bits, so the same holds for RN(q).  The quotient by
+//   s is taken with the reciprocal r = RN(1 / s) and one correction by its remainder (Markstein, IBM J. Res. Dev. 34, 1990):
+//   q0 = RN(x r), q = RN(q0 + r (x - q0 s)); the remainder is exact, so q is the quotient with a relative error of 2^-46 before
+//   its rounding.  At a border q is the border.  Off it the quotient is off by 2^-23 / 1.875 at least (s has 4 bits, so the
+//   quantity whose ulp counts has a significand of at most 1.875), 6% more than the half ulp of the border (2^-24).
+// The work is 16 values a thread, a whole block, so its maximum needs no exchange.
+#include <algorithm>
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "fp4.h"
+
+namespace b2 {
+
+namespace {
+
+// Largest |value| as bits of a non-negative float: infinities and NaN (of either sign) come out on top.
+__device__ __forceinline__ uint32_t max_bits(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t warp_max_bits(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// The scale on top for a vector whose largest magnitude has these bits.
+__device__ __forceinline__ float top_scale(uint32_t amax_bits) {
+    const uint32_t e = amax_bits & 0x7f800000u;
+    if (e == 0x7f800000u) return __uint_as_float(0x7fffffffu);
+    return __uint_as_float((e < (27u << 23) ? (27u << 23) : e) - (10u << 23));   // 27: exponent of 2^-100
+}
+// 1 / g, 0 for g = NaN
+__device__ __forceinline__ float top_inverse(float g) {
+    const uint32_t b = __float_as_uint(g);
+    return b == 0x7fffffffu ? 0.0f : __uint_as_float((254u << 23) - b);
+}
+
+// Two FP32 operations in one instruction.
+struct Pair {
+    uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// ---- plain values: blocks of 16 -------------------------------------------------------------------------------------------
+template <int TYPE>
+struct Raw {
+    static constexpr int kWords = TYPE == B2_TYPE_F32 ? 16 : 8;
+    static constexpr int kSize = TYPE == B2_TYPE_F32 ? 4 : 2;
+    uint32_t w[kWords];
+
+    // `n` values (at most 16) from element `p` on, zeros behind them; `vec`: p is on a 16-byte boundary
+    __device__ __forceinline__ void load(const uint8_t *p, int n, bool vec) {
+        if (n >= 16 && vec) {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(p + 16 * i);
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+            return;
+        }
+        if (TYPE == B2_TYPE_F32) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = i < n ? reinterpret_cast<const uint32_t *>(p)[i] : 0u;
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i)
+                w[i] = (2 * i < n ? (uint32_t)h[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)h[2 * i + 1] << 16 : 0u);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    // values 2 i and 2 i + 1
+    __device__ __forceinline__ Pair values(int i) const {
+        if (TYPE == B2_TYPE_F32) return pair(__uint_as_float(w[(2 * i) % kWords]), __uint_as_float(w[(2 * i + 1) % kWords]));
+        if (TYPE == B2_TYPE_BF16) return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        return pair(f.x, f.y);
+    }
+    __device__ __forceinline__ uint32_t amax_bits() const {
+        if (TYPE == B2_TYPE_F32) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) m = max_bits(m, w[i] & 0x7fffffffu);
+            return m;
+        }
+        uint32_t m = 0;   // 16-bit magnitudes order like their bits too
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        m = max_bits(m & 0xffffu, m >> 16);
+        if (TYPE == B2_TYPE_BF16) return m << 16;
+        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    }
+};
+
+// Code bytes and scale of a block; inv = 1 / g, 0 for a vector that is not finite.
+template <typename V>
+__device__ __forceinline__ uint32_t encode_block(V values, uint32_t amax_bits, float inv, uint2 &codes) {
+    codes = make_uint2(0u, 0u);
+    if (inv == 0.0f) return 0u;
+    const uint32_t s = cvt_e4m3x2(0.0f, div_uniform(__uint_as_float(amax_bits) * inv, 6.0f, 1.0f / 6.0f)) & 0xffu;
+    const float sf = e4m3_value((uint16_t)s);
+    const float r = s == 0u ? 0.0f : __frcp_rn(sf);
+    const Pair inv2 = pair(inv, inv), r2 = pair(r, r), ns2 = pair(-sf, -sf);
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const Pair x = mul2(values(i), inv2);
+        const Pair q = mul2(x, r2);
+        const float2 v = halves(fma2(fma2(q, ns2, x), r2, q));
+        b[i] = cvt_e2m1x2(v.y, v.x);
+    }
+    codes.x = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
+    codes.y = b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24);
+    return s;
+}
+
+// ---- by rows ----------------------------------------------------------------------------------------------------------------
+// WPR warps a row; a thread holds kHeld blocks of it, so a row of up to WPR * 32 * kHeld blocks is read once.  A longer one
+// (HELD false) is read twice, the second time out of L2 where it fits.
+constexpr int kHeld = 4;
+template <int TYPE, int WPR, bool HELD>
+__global__ void __launch_bounds__(WPR == 16 ? 512 : 256)
+k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t cols, bool vec, uint8_t *bytes, uint64_t row_bytes,
+                    uint8_t *scales, float *scale) {
+    stream_enter();
+    constexpr int kWarps = WPR == 16 ? 16 : 8, kRowsPerCta = kWarps / WPR, kThreadsPerRow = 32 * WPR;
+    __shared__ uint32_t part[kWarps];
+    const uint32_t warp = threadIdx.x >> 5, in_row = threadIdx.x % kThreadsPerRow;
+    const uint32_t row = blockIdx.x * kRowsPerCta + threadIdx.x / kThreadsPerRow;
+    const bool there = row < rows;
+    const uint32_t blocks = (cols + 15) / 16, tiles = (blocks + 3) / 4;
+    const uint8_t *src = x + (uint64_t)row * ld_bytes;
+    auto fetch = [&](Raw<TYPE> &r, uint32_t blk) {
+        if (there && blk < blocks) r.load(src + (uint64_t)blk * 16 * Raw<TYPE>::kSize, (int)min(cols - blk * 16u, 16u), vec);
+        else r.clear();
+    };
+    Raw<TYPE> held[HELD ? kHeld : 1];
+    uint32_t m = 0;
+    if (HELD) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) fetch(held[i], in_row + i * kThreadsPerRow);
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) m = max_bits(m, held[i].amax_bits());
+    } else {
+        for (uint32_t blk = in_row; blk < blocks; blk += kThreadsPerRow) {
+            fetch(held[0], blk);
+            m = max_bits(m, held[0].amax_bits());
+        }
+    }
+    m = warp_max_bits(m);
+    if (WPR > 1) {
+        if ((threadIdx.x & 31u) == 0) part[warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) m = max_bits(m, part[warp / WPR * WPR + i]);
+    }
+    const float g = top_scale(m), inv = top_inverse(g);
+    if (there && in_row == 0) scale[row] = g;
+    auto store = [&](const Raw<TYPE> &r, uint32_t blk) {
+        uint2 codes;
+        uint32_t s = encode_block([&](int i) { return r.values(i); }, r.amax_bits(), inv, codes);
+        if (there && blk < blocks) *reinterpret_cast<uint2 *>(bytes + (uint64_t)row * row_bytes + (uint64_t)blk * 8) = codes;
+        s |= __shfl_down_sync(0xffffffffu, s, 1) << 8;   // four blocks' scales, one word of a 512-byte tile
+        s |= __shfl_down_sync(0xffffffffu, s, 2) << 16;
+        if (there && (blk & 3u) == 0 && blk < tiles * 4u) *reinterpret_cast<uint32_t *>(scales + sm100_scale_offset(row, blk, tiles)) = s;
+    };
+    if (HELD) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (i * kThreadsPerRow < (int)blocks) store(held[i], in_row + i * kThreadsPerRow);
+    } else {
+        const uint32_t turns = (blocks + kThreadsPerRow - 1) / kThreadsPerRow;
+        for (uint32_t i = 0; i < turns; ++i) {
+            fetch(held[0], in_row + i * kThreadsPerRow);
+            store(held[0], in_row + i * kThreadsPerRow);
+        }
+    }
+}
+
+// ---- by columns -------------------------------------------------------------------------------------------------------------
+// Scales on top of parts of the tensor.  Rows without gaps are one row.
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+k_fp4_maxima(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint64_t cols, bool vec, float *maxima) {
+    stream_enter();
+    __shared__ uint32_t part[8];
+    uint32_t m = 0;
+    const uint64_t blocks = (cols + 15) / 16;
+    auto take = [&](const uint8_t *src, uint64_t blk) {
+        Raw<TYPE> r;
+        r.load(src + blk * 16 * Raw<TYPE>::kSize, cols - blk * 16 < 16 ? (int)(cols - blk * 16) : 16, vec);
+        m = max_bits(m, r.amax_bits());
+    };
+    if (rows == 1) {
+#pragma unroll 4
+        for (uint64_t blk = blockIdx.x * 256ull + threadIdx.x; blk < blocks; blk += gridDim.x * 256ull) take(x, blk);
+    } else {
+        for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8)
+#pragma unroll 4
+            for (uint64_t blk = threadIdx.x & 31u; blk < blocks; blk += 32) take(x + (uint64_t)row * ld_bytes, blk);
+    }
+    m = warp_max_bits(m);
+    if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 8; ++i) m = max_bits(m, part[i]);
+        maxima[blockIdx.x] = top_scale(m);
+    }
+}
+
+// A CTA transposes tiles of 128 rows x 128 columns: a warp takes 16 rows, a lane four columns of them, so that a thread holds
+// four whole blocks of the transpose and their codes only change places on the way to memory, through shared memory.
+constexpr int kTile = 128;
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+k_fp4_quantize_columns(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t cols, bool vec, uint8_t *bytes, uint64_t row_bytes,
+                       uint8_t *scales, float *scale, const float *maxima, uint32_t count) {
+    stream_enter();
+    __shared__ uint2 codes_tile[kTile * 8];   // [column][block of 16 rows], the blocks of a column in an order of its own
+    __shared__ __align__(16) uint8_t scales_tile[2 * 512];
+    __shared__ uint32_t part[8];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    uint32_t m = 0;
+    for (uint32_t i = threadIdx.x; i < count; i += 256) m = max_bits(m, __float_as_uint(maxima[i]));
+    m = warp_max_bits(m);
+    if (lane == 0) part[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_bits(m, part[i]);
+    const float g = __uint_as_float(m), inv = top_inverse(g);
+    if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = g;
+    constexpr int kSize = Raw<TYPE>::kSize;
+    const uint32_t blocks = (rows + 15) / 16, chunks = (blocks + 3) / 4;
+    const uint32_t tiles_r = (rows + kTile - 1) / kTile, tiles_c = (cols + kTile - 1) / kTile;
+    for (uint64_t tile = blockIdx.x; tile < (uint64_t)tiles_r * tiles_c; tile += gridDim.x) {
+        const uint32_t tr = (uint32_t)(tile / tiles_c), tc = (uint32_t)(tile % tiles_c);
+        const uint32_t r0 = tr * kTile + warp * 16, c0 = tc * kTile + lane * 4;
+        const uint8_t *src = x + (uint64_t)r0 * ld_bytes + (uint64_t)c0 * kSize;
+        // word [i][k]: two values (16-bit) or one (FP32) of row r0 + i
+        uint32_t w[16][kSize];
+        if (vec && c0 + 4 <= cols) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (r0 + i >= rows) {
+#pragma unroll
+                    for (int k = 0; k < kSize; ++k) w[i][k] = 0u;
+                } else if (kSize == 4) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (uint64_t)i * ld_bytes);
+                    w[i][0] = v.x; w[i][1] = v.y; w[i][2 % kSize] = v.z; w[i][3 % kSize] = v.w;
+                } else {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(src + (uint64_t)i * ld_bytes);
+                    w[i][0] = v.x; w[i][1] = v.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const bool in = r0 + i < rows;
+                const uint8_t *p = src + (uint64_t)i * ld_bytes;
+#pragma unroll
+                for (int k = 0; k < kSize; ++k) {
+                    if (kSize == 4) {
+                        w[i][k] = in && c0 + k < cols ? reinterpret_cast<const uint32_t *>(p)[k] : 0u;
+                    } else {
+                        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+                        w[i][k] = (in && c0 + 2 * k < cols ? (uint32_t)h[2 * k] : 0u) |
+                                  (in && c0 + 2 * k + 1 < cols ? (uint32_t)h[2 * k + 1] << 16 : 0u);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            Raw<TYPE> r;   // column c0 + j
+#pragma unroll
+            for (int i = 0; i < Raw<TYPE>::kWords; ++i) {
+                if (kSize == 4) r.w[i] = w[i][j % kSize];
+                else r.w[i] = __byte_perm(w[(2 * i) % 16][j >> 1], w[(2 * i + 1) % 16][j >> 1], j & 1 ? 0x7632 : 0x5410);
+            }
+            uint2 codes;
+            const uint32_t s = encode_block([&](int i) { return r.values(i); }, r.amax_bits(), inv, codes);
+            const uint32_t c = lane * 4 + j;
+            codes_tile[c * 8 + (warp ^ (lane & 7u))] = codes;
+            scales_tile[(warp >> 2) * 512 + (c & 31u) * 16 + (c >> 5) * 4 + (warp & 3u)] = (uint8_t)s;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t c = threadIdx.x / 8 + 32 * k, blk = threadIdx.x & 7u;
+            if (tc * kTile + c < cols && tr * 8 + blk < blocks)
+                *reinterpret_cast<uint2 *>(bytes + (uint64_t)(tc * kTile + c) * row_bytes + (uint64_t)(tr * 8 + blk) * 8) =
+                    codes_tile[c * 8 + (blk ^ (c >> 2 & 7u))];
+        }
+        if (threadIdx.x < 64 && tr * 2 + threadIdx.x / 32 < chunks)
+            reinterpret_cast<uint4 *>(scales + ((uint64_t)tc * chunks + tr * 2) * 512)[threadIdx.x] =
+                reinterpret_cast<const uint4 *>(scales_tile)[threadIdx.x];
+        __syncthreads();
+    }
+}
+
+// ---- reading back -----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ __half2 e2m1_values(uint32_t byte) {
+    uint32_t r;
+    asm("{ .reg .b8 t; cvt.u8.u16 t, %1; cvt.rn.f16x2.e2m1x2 %0, t; }" : "=r"(r) : "h"((uint16_t)byte));
+    return *reinterpret_cast<__half2 *>(&r);
+}
+// Values of a block: code * s is exact in FP16 (6 bits, 2^-10 .. 2688), the product with g is rounded in FP32.
+__device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, float (&v)[16]) {
+    uint32_t sh;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(sh) : "h"((uint16_t)(s | (s << 8))));
+    const __half2 s2 = *reinterpret_cast<const __half2 *>(&sh);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 f = __half22float2(__hmul2(e2m1_values((i < 4 ? codes.x : codes.y) >> (8 * (i & 3)) & 0xffu), s2));
+        v[2 * i] = f.x * g;
+        v[2 * i + 1] = f.y * g;
+    }
+}
+// `n` values (at most 16) to element `p` on; `vec`: p is on a 16-byte boundary
+template <int TYPE>
+__device__ __forceinline__ void store_block(uint8_t *p, const float (&v)[16], int n, bool vec) {
+    if (TYPE == B2_TYPE_F32) {
+        if (n >= 16 && vec) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<float4 *>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < n) reinterpret_cast<float *>(p)[i] = v[i];
+        }
+    } else {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pack_operands(v[2 * i], v[2 * i + 1], TYPE == B2_TYPE_F16);
+        if (n >= 16 && vec) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) reinterpret_cast<uint4 *>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i < n) reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        }
+    }
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+k_fp4_decode(const uint8_t *bytes, uint64_t row_bytes, const uint8_t *scales, uint32_t layout, const float *scale, bool per_row,
+             uint32_t rows, uint32_t blocks, uint32_t threads_per_row, uint8_t *out, uint64_t ld_bytes, uint32_t cols, bool vec) {
+    stream_enter();
+    const uint32_t row = blockIdx.x * (256u / threads_per_row) + threadIdx.x / threads_per_row;
+    if (row >= rows) return;
+    const uint32_t tiles = (blocks + 3) / 4;
+    const float g = scale[per_row ? row : 0];
+    for (uint32_t blk = threadIdx.x % threads_per_row; blk < blocks; blk += threads_per_row) {
+        const uint2 codes = *reinterpret_cast<const uint2 *>(bytes + (uint64_t)row * row_bytes + (uint64_t)blk * 8);
+        const uint64_t flat = (uint64_t)row * blocks + blk;
+        const uint32_t s = layout == B2_SCALES_SM100 ? scales[sm100_scale_offset(row, blk, tiles)]
+                           : layout == B2_SCALES_RAW ? scales[flat] : csf_load_scale(scales, (uint32_t)flat);
+        float v[16];
+        decode_block(codes, s, g, v);
+        store_block<TYPE>(out + (uint64_t)row * ld_bytes + (uint64_t)blk * 16 * Raw<TYPE>::kSize, v, (int)min(cols - blk * 16u, 16u), vec);
+    }
+}
+
+// ---- the paged cache --------------------------------------------------------------------------------------------------------
+// A vector's blocks lie in `group` neighbouring lanes (a power of two, at least dim / 16 of them up to a warp; vectors of more
+// than 512 values take two blocks a lane), which share its maximum.  blockIdx.y is the tensor: keys, values.
+struct CachePair {
+    b2_nvfp4_cache cache[2];
+    b2_vectors vectors[2];
+    bool vec[2];
+};
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+k_fp4_cache_write(const __grid_constant__ CachePair p, const int64_t *slots, uint32_t token_count, uint32_t group) {
+    stream_enter();
+    const b2_nvfp4_cache &c = p.cache[blockIdx.y];
+    const b2_vectors &in = p.vectors[blockIdx.y];
+    const uint64_t vector = (uint64_t)blockIdx.x * (256u / group) + threadIdx.x / group;
+    const uint32_t lane = threadIdx.x % group, blocks = c.dim / 16;
+    const uint32_t token = (uint32_t)min(vector / c.heads, (uint64_t)0xffffffffu), head = (uint32_t)(vector % c.heads);
+    int64_t slot = -1;
+    if (token < token_count) slot = slots[token];
+    const bool there = slot >= 0 && slot < (int64_t)c.pages * c.page_size;
+    const uint8_t *src = static_cast<const uint8_t *>(in.data) + (token * in.token_stride + head * in.head_stride) * Raw<TYPE>::kSize;
+    Raw<TYPE> r[2];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t blk = lane + i * group;
+        if (there && blk < blocks) r[i].load(src + (uint64_t)blk * 16 * Raw<TYPE>::kSize, 16, p.vec[blockIdx.y]);
+        else r[i].clear();
+        m = max_bits(m, r[i].amax_bits());
+    }
+    for (uint32_t o = group / 2; o > 0; o >>= 1) m = max_bits(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (!there) return;
+    const float g = top_scale(m), inv = top_inverse(g);
+    const uint64_t at = (uint64_t)slot * c.heads + head;
+    if (lane == 0) c.exponents[at] = (uint8_t)(__float_as_uint(g) >> 23);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t blk = lane + i * group;
+        if (blk >= blocks) break;
+        uint2 codes;
+        const Raw<TYPE> &block = r[i];
+        const uint32_t s = encode_block([&](int k) { return block.values(k); }, block.amax_bits(), inv, codes);
+        *reinterpret_cast<uint2 *>(c.bytes + (at * blocks + blk) * 8) = codes;
+        c.scales[at * blocks + blk] = (uint8_t)s;
+    }
+}
+
+// One CTA takes blocks of one sequence's tokens; a thread reads a block.
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+k_fp4_cache_read(const __grid_constant__ CachePair p, const int32_t *table, uint32_t table_width, const int32_t *lengths,
+                 uint32_t max_tokens, uint32_t tokens_per_cta) {
+    stream_enter();
+    const b2_nvfp4_cache &c = p.cache[blockIdx.y];
+    const b2_vectors &out = p.vectors[blockIdx.y];
+    const uint32_t sequence = blockIdx.z, blocks = c.dim / 16, per_token = c.heads * blocks;
+    const uint64_t most = min((uint64_t)max_tokens, (uint64_t)table_width * c.page_size);
+    const int32_t length = lengths[sequence];
+    const uint32_t tokens = length <= 0 ? 0u : (uint32_t)min((uint64_t)length, most);
+    const uint32_t t0 = blockIdx.x * tokens_per_cta;
+    if (t0 >= tokens) return;
+    const uint32_t work = min(tokens_per_cta, tokens - t0) * per_token;
+    for (uint32_t i = threadIdx.x; i < work; i += 256) {
+        const uint32_t t = t0 + i / per_token, rest = i % per_token, head = rest / blocks, blk = rest % blocks;
+        const int32_t page = table[(uint64_t)sequence * table_width + t / c.page_size];
+        uint2 codes = make_uint2(0u, 0u);
+        uint32_t s = 0, e = 255;
+        if (page >= 0 && (uint32_t)page < c.pages) {
+            const uint64_t at = ((uint64_t)page * c.page_size + t % c.page_size) * c.heads + head;
+            codes = *reinterpret_cast<const uint2 *>(c.bytes + (at * blocks + blk) * 8);
+            s = c.scales[at * blocks + blk];
+            e = c.exponents[at];
+        }
+        float v[16];
+        decode_block(codes, s, e == 255u ? __uint_as_float(0x7fffffffu) : e == 0u ? 0x1p-127f : __uint_as_float(e << 23), v);
+        store_block<TYPE>(static_cast<uint8_t *>(out.data) + (sequence * out.sequence_stride + t * out.token_stride + head * out.head_stride + blk * 16ull) * Raw<TYPE>::kSize,
+                          v, 16, p.vec[blockIdx.y]);
+    }
+}
+
+uint64_t type_size(uint32_t type) { return type == B2_TYPE_F32 ? 4 : 2; }
+bool aligned(const void *p, uint64_t step_bytes, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0 && step_bytes % to == 0; }
+
+#define B2_FOR_TYPE(type, F, ...)                                      \
+    if ((type) == B2_TYPE_F32) return F<B2_TYPE_F32>(__VA_ARGS__);     \
+    if ((type) == B2_TYPE_BF16) return F<B2_TYPE_BF16>(__VA_ARGS__);   \
+    return F<B2_TYPE_F16>(__VA_ARGS__);
+
+template <int TYPE>
+cudaError_t rows_impl(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s) {
+    const uint64_t ld = x.ld * Raw<TYPE>::kSize;
+    const bool vec = aligned(x.data, ld, 16);
+    const uint32_t blocks = out.cols / 16;
+    auto go = [&](auto kernel, uint32_t rows_per_cta, int threads) {
+        return overlapped_launch(kernel, dim3((x.rows + rows_per_cta - 1) / rows_per_cta), threads, 0, s, static_cast<const uint8_t *>(x.data),
+                                 ld, x.rows, x.cols, vec, out.bytes, out.row_bytes, out.scales, out.scale);
+    };
+    if (blocks <= 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 1, true>, 8, 256);
+    if (blocks <= 4 * 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 4, true>, 2, 256);
+    if (blocks <= 16 * 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 16, true>, 1, 512);
+    return go(k_fp4_quantize_rows<TYPE, 16, false>, 1, 512);
+}
+template <int TYPE>
+cudaError_t maxima_impl(const b2_matrix &x, float *maxima, uint32_t *count, int sm_count, cudaStream_t s) {
+    const uint64_t ld = x.ld * Raw<TYPE>::kSize;
+    const bool flat = x.ld == x.cols || x.rows == 1;
+    const uint32_t rows = flat ? 1u : x.rows;
+    const uint64_t cols = flat ? (uint64_t)x.rows * x.cols : x.cols;
+    // the warps' worth of work there is, up to 8 CTAs an SM
+    const uint64_t warps = flat ? (cols + 511) / 512 : rows;
+    const uint32_t grid = (uint32_t)std::min<uint64_t>((warps + 7) / 8, std::min(B2_NVFP4_MAXIMA, sm_count * 6));
+    *count = grid;
+    return overlapped_launch(k_fp4_maxima<TYPE>, dim3(grid), 256, 0, s, static_cast<const uint8_t *>(x.data), ld, rows, cols,
+                             aligned(x.data, rows == 1 ? 0 : ld, 16), maxima);
+}
+template <int TYPE>
+cudaError_t columns_impl(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count, int sm_count, cudaStream_t s) {
+    const uint64_t ld = x.ld * Raw<TYPE>::kSize;
+    const uint64_t tiles = (uint64_t)((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
+    const uint32_t grid = (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sm_count * 4);
+    return overlapped_launch(k_fp4_quantize_columns<TYPE>, dim3(grid), 256, 0, s, static_cast<const uint8_t *>(x.data), ld, x.rows, x.cols,
+                             aligned(x.data, ld, 4 * Raw<TYPE>::kSize), out.bytes, out.row_bytes, out.scales, out.scale, maxima, count);
+}
+template <int TYPE>
+cudaError_t decode_impl(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s) {
+    const uint64_t ld = out.ld * Raw<TYPE>::kSize;
+    const uint32_t blocks = in.cols / 16;
+    uint32_t tpr = 1;
+    while (tpr < blocks && tpr < 256) tpr *= 2;
+    const uint32_t per_cta = 256 / tpr;
+    return overlapped_launch(k_fp4_decode<TYPE>, dim3((in.rows + per_cta - 1) / per_cta), 256, 0, s, static_cast<const uint8_t *>(in.bytes),
+                             in.row_bytes, static_cast<const uint8_t *>(in.scales), layout, static_cast<const float *>(in.scale),
+                             in.scale_count != 1, in.rows, blocks, tpr, static_cast<uint8_t *>(out.data), ld, out.cols, aligned(out.data, ld, 16));
+}
+CachePair cache_pair(const b2_nvfp4_cache *caches, const b2_vectors *vectors, uint32_t count) {
+    CachePair p = {};
+    for (uint32_t i = 0; i < count; ++i) {
+        p.cache[i] = caches[i];
+        p.vectors[i] = vectors[i];
+        const uint64_t size = type_size(vectors[i].type);
+        const uint64_t strides = (vectors[i].sequence_stride | vectors[i].token_stride | vectors[i].head_stride) * size;
+        p.vec[i] = aligned(vectors[i].data, strides, 16);
+    }
+    return p;
+}
+template <int TYPE>
+cudaError_t write_impl(const CachePair &p, uint32_t count, const int64_t *slots, uint32_t token_count, cudaStream_t s) {
+    uint32_t blocks = 0, heads = 0, group = 1;
+    for (uint32_t i = 0; i < count; ++i) {
+        blocks = std::max(blocks, p.cache[i].dim / 16);
+        heads = std::max(heads, p.cache[i].heads);
+    }
+    while (group < blocks && group < 32) group *= 2;
+    const uint64_t grid = ((uint64_t)token_count * heads + 256 / group - 1) / (256 / group);
+    if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
+    return overlapped_launch(k_fp4_cache_write<TYPE>, dim3((unsigned)grid, count), 256, 0, s, p, slots, token_count, group);
+}
+template <int TYPE>
+cudaError_t read_impl(const CachePair &p, uint32_t count, const int32_t *table, uint32_t table_width, const int32_t *lengths,
+                      uint32_t sequences, uint32_t max_tokens, cudaStream_t s) {
+    uint32_t per_token = 0;
+    for (uint32_t i = 0; i < count; ++i) per_token = std::max(per_token, p.cache[i].heads * (p.cache[i].dim / 16));
+    const uint32_t tokens = std::max(1u, 1024u / per_token);   // about four blocks a thread
+    return overlapped_launch(k_fp4_cache_read<TYPE>, dim3((max_tokens + tokens - 1) / tokens, count, sequences), 256, 0, s, p, table,
+                             table_width, lengths, max_tokens, tokens);
+}
+
+}  // namespace
+
+cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s) {
+    B2_FOR_TYPE(x.type, rows_impl, x, out, s)
+}
+cudaError_t launch_fp4_maxima(const b2_matrix &x, float *maxima, uint32_t *count, int sm_count, cudaStream_t s) {
+    B2_FOR_TYPE(x.type, maxima_impl, x, maxima, count, sm_count, s)
+}
+cudaError_t launch_fp4_quantize_columns(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count, int sm_count,
+                                        cudaStream_t s) {
+    B2_FOR_TYPE(x.type, columns_impl, x, out, maxima, count, sm_count, s)
+}
+cudaError_t launch_fp4_decode(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s) {
+    B2_FOR_TYPE(out.type, decode_impl, in, layout, out, s)
+}
+cudaError_t launch_fp4_cache_write(const b2_nvfp4_cache *caches, const b2_vectors *tokens, uint32_t count, const int64_t *slots,
+                                   uint32_t token_count, cudaStream_t s) {
+    const CachePair p = cache_pair(caches, tokens, count);
+    B2_FOR_TYPE(tokens[0].type, write_impl, p, count, slots, token_count, s)
+}
+cudaError_t launch_fp4_cache_read(const b2_nvfp4_cache *caches, const b2_vectors *out, uint32_t count, const int32_t *table,
+                                  uint32_t table_width, const int32_t *lengths, uint32_t sequences, uint32_t max_tokens, cudaStream_t s) {
+    const CachePair p = cache_pair(caches, out, count);
+    B2_FOR_TYPE(out[0].type, read_impl, p, count, table, table_width, lengths, sequences, max_tokens, s)
+}
+
+}  // namespace b2

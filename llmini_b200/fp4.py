@@ -1,0 +1,300 @@
+"""The 4-bit operators beside the requantised weights, over the C ABI of include/llmini_b200_fp4.h.
+
+Activations and gradients quantised to NVFP4 by rows or by columns, the product of NVFP4 operands, the linear layer and its
+gradients, reading 4-bit tensors back, and a paged cache of keys and values.  Tensors are torch CUDA tensors used purely as
+device buffers; every call enqueues its work on the current stream of the current device, which has to hold all of them.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass, field
+
+import torch
+
+from . import _ffi
+from ._ffi import SCALES_CSF, SCALES_RAW, SCALES_SM100, check
+from .nvfp4 import Nvfp4Tensor, _stream
+
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+NVFP4_MAXIMA = 1024
+_TYPES = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+
+
+class Matrix(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("ld", C.c_uint64), ("rows", C.c_uint32), ("cols", C.c_uint32), ("type", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
+class Operand(C.Structure):
+    _fields_ = [("bytes", C.c_void_p), ("scales", C.c_void_p), ("scale", C.c_void_p), ("row_bytes", C.c_uint64), ("rows", C.c_uint32),
+                ("cols", C.c_uint32), ("scale_count", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class LinearGradients(C.Structure):
+    _fields_ = [("grad", Matrix), ("x", Matrix), ("weight_t", Operand), ("grad_x", Matrix), ("grad_weight", Matrix), ("grad_rows", Operand),
+                ("grad_columns", Operand), ("x_columns", Operand), ("d_maxima", C.c_void_p), ("accumulate", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+class Cache(C.Structure):
+    _fields_ = [("bytes", C.c_void_p), ("scales", C.c_void_p), ("exponents", C.c_void_p), ("pages", C.c_uint32), ("page_size", C.c_uint32),
+                ("heads", C.c_uint32), ("dim", C.c_uint32)]
+
+
+class Vectors(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("sequence_stride", C.c_uint64), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64),
+                ("type", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+_declared = False
+
+
+def _lib() -> C.CDLL:
+    global _declared
+    L = _ffi.lib()
+    if not _declared:
+        vp, u32, i = C.c_void_p, C.c_uint32, C.c_int
+        sig = {
+            "b2_nvfp4_quantize_rows": [vp, vp, vp],
+            "b2_nvfp4_quantize_columns": [vp, vp, vp, vp],
+            "b2_nvfp4_decode": [vp, u32, vp, vp],
+            "b2_nvfp4_matmul": [vp, vp, vp, vp, u32, vp],
+            "b2_nvfp4_linear_forward": [vp, vp, vp, vp, vp, vp],
+            "b2_nvfp4_linear_backward": [vp, vp],
+            "b2_nvfp4_status": [vp],
+            "b2_nvfp4_cache_write": [vp, vp, u32, vp, u32, vp],
+            "b2_nvfp4_cache_read": [vp, vp, u32, vp, u32, vp, u32, u32, vp],
+        }
+        for name, args in sig.items():
+            fn = getattr(L, name)
+            fn.restype, fn.argtypes = i, args
+        _declared = True
+    return L
+
+
+def _refuse(what: str):
+    raise ValueError(what)
+
+
+def _here(t: torch.Tensor) -> int:
+    """The address of a tensor of the current device."""
+    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+        _refuse(f"a tensor on {t.device}: the call works on the current CUDA device")
+    return t.data_ptr()
+
+
+def _matrix(t: torch.Tensor) -> Matrix:
+    if t.dim() != 2 or t.dtype not in _TYPES:
+        _refuse(f"a matrix of FP32, BF16 or F16 is wanted, not {tuple(t.shape)} of {t.dtype}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        _refuse("a row's values have to lie side by side")
+    ld = t.stride(0) if rows > 1 else cols
+    if ld < cols:
+        _refuse("rows overlap")
+    return Matrix(_here(t), ld, rows, cols, _TYPES[t.dtype], 0)
+
+
+def _floats(t: torch.Tensor, count: int, what: str) -> int:
+    if t.dtype != torch.float32 or t.numel() < count or not t.is_contiguous():
+        _refuse(f"{what}: {count} contiguous FP32 values are wanted")
+    return _here(t)
+
+
+def _up(n: int, step: int) -> int:
+    return -(-n // step) * step
+
+
+@dataclass
+class Nvfp4Operand:
+    """A matrix in NVFP4 as the product reads it: codes [rows, row_bytes] (two a byte, k / 2 of a row's bytes), block scales in the
+    tensor cores' layout (SCALES_SM100), and the scale on top, one or one a row.  k: the values of a row, a multiple of 16."""
+    bytes: torch.Tensor
+    scales: torch.Tensor
+    scale: torch.Tensor
+    rows: int
+    k: int
+    c: Operand = field(init=False, repr=False)
+
+    def __post_init__(self):
+        b = self.bytes
+        if b.dtype != torch.uint8 or b.dim() != 2 or b.shape[0] != self.rows or (b.shape[1] > 1 and b.stride(1) != 1):
+            _refuse("codes: uint8 [rows, bytes of a row]")
+        row_bytes = b.stride(0) if self.rows > 1 else _up(b.shape[1], 16)
+        if self.k % 16 or self.k <= 0 or b.shape[1] < self.k // 2 or row_bytes % 16:
+            _refuse("a row: k values, a multiple of 16, on a 16-byte boundary")
+        if self.scales.dtype != torch.uint8 or not self.scales.is_contiguous() or self.scales.numel() < _up(self.rows, 128) * _up(self.k // 16, 4):
+            _refuse("scales: a contiguous buffer of sm100_scales_bytes(rows, k) bytes")
+        n = self.scale.numel()
+        if self.scale.dtype != torch.float32 or not self.scale.is_contiguous() or n not in (1, self.rows):
+            _refuse("scale: FP32, one or one a row")
+        if self.rows and (b.data_ptr() % 16 or self.scales.data_ptr() % 16):
+            _refuse("codes and scales start on 16-byte boundaries")
+        if not (b.device == self.scales.device == self.scale.device) or not b.is_cuda:
+            _refuse("an operand lies on one CUDA device")
+        self.device_index = b.device.index
+        self.c = Operand(b.data_ptr(), self.scales.data_ptr(), self.scale.data_ptr(), row_bytes, self.rows, self.k, n, 0)
+
+    @staticmethod
+    def empty(rows: int, k: int, per_row: bool = True, device="cuda") -> "Nvfp4Operand":
+        """Memory for `rows` rows of k values, rounded up to a multiple of 16: what the quantisers write."""
+        k = max(_up(k, 16), 16)
+        return Nvfp4Operand(torch.empty(rows, _up(k // 2, 16), dtype=torch.uint8, device=device),
+                            torch.zeros(max(_up(rows, 128) * _up(k // 16, 4), 16), dtype=torch.uint8, device=device),
+                            torch.empty(rows if per_row else 1, dtype=torch.float32, device=device), rows, k)
+
+    @staticmethod
+    def from_tensor(t: Nvfp4Tensor) -> "Nvfp4Operand":
+        """A requantised weight [rows][k] as it lies, its scales in SCALES_SM100 (a plan of that layout, or `scales_to_sm100`);
+        k has to be a multiple of 32, so that rows start on 16-byte boundaries."""
+        if t.scale_layout != SCALES_SM100:
+            _refuse("scales in SCALES_SM100 are wanted: see scales_to_sm100")
+        return Nvfp4Operand(t.bytes.view(t.rows, t.k // 2), t.scales, t.global_scale, t.rows, t.k)
+
+
+class Nvfp4LinearScratch:
+    """Memory of a linear layer's calls on `tokens` rows: its quantised activations, with `backward` also what the gradients
+    need.  Calls that may run at the same time, captured ones too, each need their own."""
+
+    def __init__(self, tokens: int, inputs: int, outputs: int, backward: bool = False, device="cuda"):
+        self.rows = None if backward else Nvfp4Operand.empty(tokens, inputs, device=device)
+        self.backward = backward
+        if backward:
+            self.grad_rows = Nvfp4Operand.empty(tokens, outputs, device=device)
+            self.grad_columns = Nvfp4Operand.empty(outputs, tokens, per_row=False, device=device)
+            self.x_columns = Nvfp4Operand.empty(inputs, tokens, per_row=False, device=device)
+            self.maxima = torch.empty(2 * NVFP4_MAXIMA, dtype=torch.float32, device=device)
+
+
+@dataclass
+class Nvfp4PagedCache:
+    """Keys and values in pages: for each, codes [pages, page_size, heads, dim / 2], block scales [.., dim / 16] and exponents
+    [pages, page_size, heads], all uint8 and contiguous.  `value` may be None: a cache of one tensor."""
+    key: tuple
+    value: tuple | None = None
+    c: object = field(init=False, repr=False)
+
+    def __post_init__(self):
+        sides = [self.key] + ([self.value] if self.value is not None else [])
+        self.c = (Cache * len(sides))()
+        for i, (codes, scales, exponents) in enumerate(sides):
+            pages, page_size, heads, half = codes.shape
+            shapes = (codes.shape, scales.shape, exponents.shape) == ((pages, page_size, heads, half), (pages, page_size, heads, half // 8), (pages, page_size, heads))
+            if half % 8 or not shapes or any(t.dtype != torch.uint8 or not t.is_contiguous() for t in (codes, scales, exponents)):
+                _refuse("a cache: uint8 [pages, page_size, heads, dim / 2], [.., dim / 16], [pages, page_size, heads]")
+            if not codes.is_cuda or not (codes.device == scales.device == exponents.device == sides[0][0].device):
+                _refuse("a cache lies on one CUDA device")
+            self.c[i] = Cache(codes.data_ptr(), scales.data_ptr(), exponents.data_ptr(), pages, page_size, heads, half * 2)
+        self.device_index = sides[0][0].device.index
+
+    @staticmethod
+    def empty(pages: int, page_size: int, heads: int, dim: int, value_dim: int | None = None, device="cuda") -> "Nvfp4PagedCache":
+        def side(d):
+            return tuple(torch.zeros(pages, page_size, heads, *more, dtype=torch.uint8, device=device) for more in ((d // 2,), (d // 16,), ()))
+        return Nvfp4PagedCache(side(dim), side(value_dim or dim))
+
+
+class Nvfp4LinearModule:
+    """The entry points, named after those of the library."""
+
+    def __init__(self):
+        self._lib = _lib()
+
+    @staticmethod
+    def _ref(o):
+        if o.device_index != torch.cuda.current_device():
+            _refuse("an operand of another device than the current one")
+        return C.byref(o.c)
+
+    def quantize_rows(self, x: torch.Tensor, out: Nvfp4Operand) -> None:
+        check(self._lib.b2_nvfp4_quantize_rows(C.byref(_matrix(x)), self._ref(out), _stream()), "nvfp4_quantize_rows")
+
+    def quantize_columns(self, x: torch.Tensor, out: Nvfp4Operand, maxima: torch.Tensor) -> None:
+        """The transpose of x; `maxima`: scratch of NVFP4_MAXIMA FP32 values."""
+        check(self._lib.b2_nvfp4_quantize_columns(C.byref(_matrix(x)), self._ref(out), _floats(maxima, NVFP4_MAXIMA, "maxima"), _stream()),
+              "nvfp4_quantize_columns")
+
+    def decode(self, operand, out: torch.Tensor) -> None:
+        """The values of an Nvfp4Operand, or of an Nvfp4Tensor of any scale layout, in out's type."""
+        layout, c = SCALES_SM100, None
+        if isinstance(operand, Nvfp4Tensor):
+            t, layout = operand, operand.scale_layout
+            if (t.k // 2) % 16 and t.rows > 1:
+                _refuse("rows of k values start on 16-byte boundaries where k is a multiple of 32")
+            need = _up(t.rows, 128) * _up(t.k // 16, 4) if layout == SCALES_SM100 else t.rows * t.k // 16 if layout == SCALES_RAW else 128
+            if t.bytes.numel() < t.rows * t.k // 2 or t.scales.numel() < need:
+                _refuse("an Nvfp4Tensor with too little memory for its rows and k")
+            c = C.byref(Operand(_here(t.bytes), _here(t.scales), _here(t.global_scale), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
+        check(self._lib.b2_nvfp4_decode(c or self._ref(operand), layout, C.byref(_matrix(out)), _stream()), "nvfp4_decode")
+
+    def _bias(self, bias, n):
+        return None if bias is None else _floats(bias, n, "bias")
+
+    def matmul(self, a: Nvfp4Operand, b: Nvfp4Operand, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False) -> None:
+        """out [a.rows, b.rows] = a b^T (+ bias) (+ out, FP32 only)."""
+        check(self._lib.b2_nvfp4_matmul(self._ref(a), self._ref(b), C.byref(_matrix(out)), self._bias(bias, b.rows), int(accumulate), _stream()),
+              "nvfp4_matmul")
+
+    def linear_forward(self, x: torch.Tensor, weight: Nvfp4Operand, out: torch.Tensor, scratch: Nvfp4LinearScratch,
+                       bias: torch.Tensor | None = None) -> None:
+        """out [tokens, outputs] = Q(x) weight^T (+ bias)."""
+        if scratch.rows is None:
+            _refuse("scratch of the backward pass")
+        check(self._lib.b2_nvfp4_linear_forward(C.byref(_matrix(x)), self._ref(weight), C.byref(_matrix(out)), self._bias(bias, weight.rows),
+                                                self._ref(scratch.rows), _stream()), "nvfp4_linear_forward")
+
+    def linear_backward(self, grad: torch.Tensor, x: torch.Tensor | None, weight_t: Nvfp4Operand | None, grad_x: torch.Tensor | None,
+                        grad_weight: torch.Tensor | None, scratch: Nvfp4LinearScratch, accumulate: bool = False) -> None:
+        """grad_x [tokens, inputs] and grad_weight [outputs, inputs] (FP32) of linear_forward; either may be None.  weight_t: the
+        transposed weight, quantised along the outputs (quantize_columns of the master weights)."""
+        if not scratch.backward:
+            _refuse("scratch of the forward pass")
+        g = LinearGradients()
+        g.grad = _matrix(grad)
+        if grad_x is not None:
+            self._ref(weight_t)
+            g.weight_t, g.grad_x = weight_t.c, _matrix(grad_x)
+        if grad_weight is not None:
+            g.x, g.grad_weight = _matrix(x), _matrix(grad_weight)
+        self._ref(scratch.grad_rows)
+        g.grad_rows, g.grad_columns, g.x_columns = scratch.grad_rows.c, scratch.grad_columns.c, scratch.x_columns.c
+        g.d_maxima, g.accumulate = scratch.maxima.data_ptr(), int(accumulate)
+        check(self._lib.b2_nvfp4_linear_backward(C.byref(g), _stream()), "nvfp4_linear_backward")
+
+    def status(self) -> int:
+        """0, or ERROR_LAUNCH_TIMEOUT if a bounded device wait of a product ran out since the last call (synchronises)."""
+        return int(self._lib.b2_nvfp4_status(_stream()))
+
+    def _sides(self, cache: Nvfp4PagedCache, tensors, dims: int):
+        tensors = [t for t in tensors if t is not None]
+        if len(tensors) != len(cache.c):
+            _refuse("one tensor for each side of the cache")
+        if cache.device_index != torch.cuda.current_device():
+            _refuse("a cache of another device than the current one")
+        v = (Vectors * len(tensors))()
+        for i, t in enumerate(tensors):
+            c = cache.c[i]
+            if t.dim() != dims or t.dtype not in _TYPES or t.dtype != tensors[0].dtype or t.shape[:-2] != tensors[0].shape[:-2]:
+                _refuse("keys and values: tensors of one type and length")
+            if t.shape[-2:] != (c.heads, c.dim) or t.stride(-1) != 1 or min(t.stride()) < 0:
+                _refuse("vectors of the cache's heads and size, their values side by side")
+            v[i] = Vectors(_here(t), t.stride(0) if dims == 4 else 0, t.stride(-3), t.stride(-2), _TYPES[t.dtype], 0)
+        return v, tensors[0]
+
+    def cache_write(self, cache: Nvfp4PagedCache, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor | None = None) -> None:
+        """key, value [tokens, heads, dim] into slots int64 [tokens] (page * page_size + place; others leave a token out)."""
+        v, first = self._sides(cache, (key, value), 3)
+        if slots.dtype != torch.int64 or slots.shape != first.shape[:1] or not slots.is_contiguous():
+            _refuse("slots: int64 [tokens]")
+        check(self._lib.b2_nvfp4_cache_write(cache.c, v, len(v), _here(slots), first.shape[0], _stream()), "nvfp4_cache_write")
+
+    def cache_read(self, cache: Nvfp4PagedCache, table: torch.Tensor, lengths: torch.Tensor, key: torch.Tensor,
+                   value: torch.Tensor | None = None) -> None:
+        """The first lengths[b] tokens of every sequence b, whose pages table [sequences, pages of a sequence] lists, into key,
+        value [sequences, tokens, heads, dim]; what lies behind them is left as it is.  table, lengths: int32."""
+        v, first = self._sides(cache, (key, value), 4)
+        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] != first.shape[0]:
+            _refuse("table: int32 [sequences, pages of a sequence]")
+        if lengths.dtype != torch.int32 or lengths.shape != first.shape[:1] or not lengths.is_contiguous():
+            _refuse("lengths: int32 [sequences]")
+        check(self._lib.b2_nvfp4_cache_read(cache.c, v, len(v), _here(table), table.shape[1], _here(lengths), first.shape[0], first.shape[1],
+                                            _stream()), "nvfp4_cache_read")

@@ -23,6 +23,8 @@ use std::cell::Cell;
 
 use cuda_core::{CudaStream, DeviceBuffer, DriverError};
 
+pub mod fp4;
+
 pub mod ffi {
     //! Mirror of include/llmini_b200.h: same names, same field order.
     use std::ffi::c_void;

@@ -1,0 +1,180 @@
+"""The 4-bit operators without a GPU: what the header declares is exported and mirrored, what is wrong is refused before anything
+is launched, and the plain definition that the kernels are tested against does what it says."""
+import ctypes as C
+import os
+import re
+
+import numpy as np
+import pytest
+import torch
+
+import llmini_b200 as b2
+from llmini_b200 import _ffi, fp4
+from tests import fp4_plain as plain
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "llmini_b200_fp4.h")).read(), flags=re.S)
+SHIM = re.sub(r"//[^\n]*", "", open(os.path.join(ROOT, "rust-shim", "src", "fp4.rs")).read())
+INVALID = _ffi.ERROR_INVALID_VALUE
+AT = 4096   # an address that is never looked at
+
+
+def structs(text):
+    return {m.group(1): [re.findall(r"(\w+)\s*$", part.strip())[0] for decl in m.group(2).split(";") if decl.strip() for part in decl.split(",")]
+            for m in re.finditer(r"typedef\s+struct\s+(b2_\w+)\s*\{(.*?)\}\s*\1\s*;", text, flags=re.S)}
+
+
+def test_exports_and_mirrors():
+    declared = {m.group(1): m.group(2).count(",") + 1 for m in re.finditer(r"\b(b2_nvfp4_\w+)\s*\(([^;{}]*?)\)\s*;", HEADER, flags=re.S)}
+    assert len(declared) == 9
+    for name in declared:
+        fn = getattr(fp4._lib(), name)
+        assert len(fn.argtypes) == declared[name], name
+    bound = {m.group(1): len([a for a in m.group(2).split(",") if a.strip()]) for m in re.finditer(r"pub fn (b2_nvfp4_\w+)\s*\((.*?)\)\s*->", SHIM, flags=re.S)}
+    assert bound == declared
+    mirrors = {"b2_matrix": fp4.Matrix, "b2_nvfp4_operand": fp4.Operand, "b2_nvfp4_linear_gradients": fp4.LinearGradients, "b2_nvfp4_cache": fp4.Cache,
+               "b2_vectors": fp4.Vectors}
+    h = structs(HEADER)
+    assert set(h) == set(mirrors)
+    for name, fields in h.items():
+        assert [f for f, _ in mirrors[name]._fields_] == fields, name
+        body = re.search(rf"#\[repr\(C\)\][^{{;]*?pub struct {name}\s*\{{(.*?)\n\}}", SHIM, flags=re.S).group(1)
+        assert re.findall(r"pub (?:r#)?(\w+)\s*:", body) == fields, name
+    assert [C.sizeof(t) for t in mirrors.values()] == [32, 48, 336, 40, 40]
+    assert int(re.search(r"#define B2_NVFP4_MAXIMA (\d+)", HEADER).group(1)) == b2.NVFP4_MAXIMA == int(re.search(r"B2_NVFP4_MAXIMA: usize = (\d+)", SHIM).group(1))
+    for name, value in re.findall(r"(B2_TYPE_\w+) = (\d)", HEADER):
+        assert re.search(rf"pub const {name}: u32 = {value};", SHIM), name
+
+
+def matrix(rows, cols, ld=None, type=fp4.TYPE_BF16, data=AT):
+    return fp4.Matrix(data, cols if ld is None else ld, rows, cols, type, 0)
+
+
+def operand(rows, cols, count=None, row_bytes=None, data=AT):
+    return fp4.Operand(data, data, data, -(-cols // 32) * 16 if row_bytes is None else row_bytes, rows, cols, rows if count is None else count, 0)
+
+
+def with_field(struct, **fields):
+    for name, v in fields.items():
+        setattr(struct, name, v)
+    return struct
+
+
+BAD_MATRICES = [matrix(4, 64, data=None), matrix(4, 64, ld=63), matrix(4, 64, type=3), matrix(4, 64, data=AT + 1), with_field(matrix(4, 64), reserved=1),
+                matrix(4, 64, ld=1 << 40), matrix(65535 * 128 + 1, 64)]
+BAD_OPERANDS = [operand(4, 64, data=None), operand(4, 64, data=AT + 8), operand(4, 64, row_bytes=40), operand(4, 64, row_bytes=16), operand(4, 64, count=3),
+                operand(4, 72), with_field(operand(4, 64), reserved=7), operand(4, 64, row_bytes=1 << 40)]
+
+
+def test_quantisers_refuse():
+    L = fp4._lib()
+    rows = lambda x, o: L.b2_nvfp4_quantize_rows(C.byref(x) if x else None, C.byref(o) if o else None, None)
+    columns = lambda x, o, maxima=AT: L.b2_nvfp4_quantize_columns(C.byref(x) if x else None, C.byref(o) if o else None, maxima, None)
+    good = (matrix(4, 64), operand(4, 64))
+    assert rows(None, good[1]) == rows(good[0], None) == INVALID
+    for bad in BAD_MATRICES:
+        assert rows(bad, good[1]) == INVALID, bad.ld
+        assert columns(bad, operand(64, 16, 1)) == INVALID
+    for bad in BAD_OPERANDS:
+        assert rows(good[0], bad) == INVALID
+    for o in (operand(5, 64), operand(4, 80), operand(4, 64, 1)):
+        assert rows(good[0], o) == INVALID
+    for o in (operand(64, 32, 1), operand(63, 16, 1), operand(64, 16), operand(64, 16, 1, data=None)):
+        assert columns(good[0], o) == INVALID
+    assert columns(good[0], operand(64, 16, 1), None) == columns(good[0], operand(64, 16, 1), AT + 2) == INVALID
+    assert columns(matrix(0, 64), operand(64, 16, 1)) == INVALID
+    assert rows(matrix(0, 64), operand(0, 64)) == 0
+
+
+def test_products_refuse():
+    L = fp4._lib()
+    mm = lambda a, b, c, bias=None, acc=0: L.b2_nvfp4_matmul(C.byref(a), C.byref(b), C.byref(c), bias, acc, None)
+    a, b, c = operand(4, 64), operand(8, 64, 1), matrix(4, 8, type=fp4.TYPE_F32)
+    for bad in BAD_OPERANDS:
+        assert mm(bad, b, c) == INVALID and mm(a, bad, matrix(4, bad.rows)) == INVALID
+    for bad in BAD_MATRICES:
+        assert mm(operand(4, 64), operand(64, 64, 1), bad) == INVALID
+    assert mm(a, operand(8, 48, 1), c) == mm(a, b, matrix(4, 9)) == mm(a, b, matrix(5, 8)) == INVALID
+    assert mm(a, b, c, bias=AT + 2) == mm(a, b, c, acc=2) == mm(a, b, matrix(4, 8), acc=1) == INVALID
+    assert mm(operand(0, 64), b, matrix(0, 8)) == mm(a, operand(0, 64, 1), matrix(4, 0)) == 0
+    fw = lambda x, w, y, s: L.b2_nvfp4_linear_forward(C.byref(x), C.byref(w), C.byref(y), None, C.byref(s), None)
+    assert fw(matrix(4, 64), b, matrix(4, 8), operand(4, 64, 1)) == INVALID
+    assert fw(matrix(4, 60), b, matrix(4, 8), operand(4, 80)) == fw(matrix(4, 80), b, matrix(4, 8), operand(4, 80)) == INVALID
+    assert fw(matrix(0, 64), b, matrix(0, 8), operand(0, 64)) == 0
+
+    def bw(**fields):
+        g = fp4.LinearGradients(matrix(20, 8), matrix(20, 64), operand(64, 16, 1), matrix(20, 64), matrix(8, 64, type=fp4.TYPE_F32), operand(20, 16),
+                                operand(8, 32, 1), operand(64, 32, 1), AT, 0, 0)
+        return L.b2_nvfp4_linear_backward(C.byref(with_field(g, **fields)), None)
+    for fields in (dict(grad=matrix(20, 0)), dict(x=matrix(19, 64)), dict(weight_t=operand(64, 32, 1)), dict(grad_x=matrix(20, 63)), dict(d_maxima=None),
+                   dict(grad_weight=matrix(8, 64)), dict(grad_weight=matrix(64, 8, type=fp4.TYPE_F32)), dict(grad_rows=operand(20, 16, 1)),
+                   dict(grad_columns=operand(8, 32)), dict(x_columns=operand(64, 16, 1)), dict(accumulate=2), dict(reserved=1)):
+        assert bw(**fields) == INVALID, fields
+
+
+def test_decode_refuses():
+    L = fp4._lib()
+    dec = lambda o, m, layout=2: L.b2_nvfp4_decode(C.byref(o), layout, C.byref(m), None)
+    for bad in BAD_OPERANDS:
+        assert dec(bad, matrix(4, 64)) == INVALID
+    for bad in BAD_MATRICES:
+        assert dec(operand(4, 64), bad) == INVALID
+    assert dec(operand(4, 64), matrix(4, 48)) == dec(operand(4, 64), matrix(3, 64)) == dec(operand(4, 64), matrix(4, 64), 3) == INVALID
+    assert dec(operand(4, 64), matrix(4, 64), 0) == INVALID                                   # CSF: whole 128-value pieces
+    assert dec(operand(65536, 1 << 21, 1), matrix(65536, 1 << 21), 0) == INVALID              # and 32-bit group numbers
+
+
+def test_cache_refuses():
+    L = fp4._lib()
+    cache = lambda **f: (fp4.Cache * 1)(with_field(fp4.Cache(AT, AT, AT, 4, 16, 2, 64), **f))
+    vectors = lambda **f: (fp4.Vectors * 1)(with_field(fp4.Vectors(AT, 4096, 128, 64, fp4.TYPE_BF16, 0), **f))
+    write = lambda c, v, count=1, slots=AT, n=5: L.b2_nvfp4_cache_write(c, v, count, slots, n, None)
+    read = lambda c, v, count=1, table=AT, lengths=AT, b=2, n=30: L.b2_nvfp4_cache_read(c, v, count, table, 2, lengths, b, n, None)
+    for f in (dict(bytes=None), dict(bytes=AT + 4), dict(scales=None), dict(exponents=None), dict(page_size=0), dict(heads=0), dict(dim=40), dict(dim=0),
+              dict(dim=1040), dict(heads=65536)):
+        assert write(cache(**f), vectors()) == read(cache(**f), vectors()) == INVALID, f
+    for f in (dict(data=None), dict(data=AT + 1), dict(type=3), dict(reserved=1), dict(token_stride=1 << 40)):
+        assert write(cache(), vectors(**f)) == read(cache(), vectors(**f)) == INVALID, f
+    assert write(cache(), vectors(), 0) == write(cache(), vectors(), 3) == write(cache(), vectors(), slots=None) == write(cache(), vectors(), slots=AT + 4) == INVALID
+    assert read(cache(), vectors(), 0) == read(cache(), vectors(), table=None) == read(cache(), vectors(), lengths=AT + 2) == read(cache(), vectors(), b=65536) == INVALID
+    two = (fp4.Vectors * 2)(vectors()[0], vectors(type=fp4.TYPE_F16)[0])
+    assert write((fp4.Cache * 2)(cache()[0], cache()[0]), two, 2) == INVALID
+    assert write(cache(), vectors(), n=0) == read(cache(), vectors(), b=0) == read(cache(), vectors(), n=0) == 0
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU failure mode")
+def test_calls_fail_loudly_without_a_gpu():
+    L = fp4._lib()
+    assert L.b2_nvfp4_quantize_rows(C.byref(matrix(4, 64)), C.byref(operand(4, 64)), None) not in (0, INVALID)
+    assert L.b2_nvfp4_matmul(C.byref(operand(4, 64)), C.byref(operand(8, 64, 1)), C.byref(matrix(4, 8)), None, 0, None) not in (0, INVALID)
+    with pytest.raises(ValueError):
+        b2.Nvfp4LinearModule().quantize_rows(torch.zeros(4, 64), None)
+
+
+def test_plain_definition():
+    x = np.array([[6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.25, -5.0] + [0.0] * 8])
+    codes, s, g = plain.quantise(x)
+    assert g[0] == 2.0 ** -8 and s[0, 0] == 0x78 and plain.e4m3_grid()[0x78] == 256 and codes.shape == (1, 32)   # 1 / 2^-8
+    assert codes[0, :10].tolist() == [7, 0, 2, 2, 4, 4, 6, 6, 8, 14]
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((5, 100)) * np.exp2(rng.integers(-20, 20, (5, 1)))
+    codes, s, g = plain.quantise(x)
+    err = np.abs(plain.values(codes, s, g)[:, :100] - x)
+    step = np.repeat(plain.e4m3_grid()[s] * g[:, None], 16, 1)[:, :100]
+    assert (err <= 1.4 * step).all()   # half the widest step, and what saturates: 6 (1 + 1/16) - 6
+    assert np.array_equal(plain.untiled(plain.tiled(s), 5, 7)[0], s) and np.array_equal(plain.unpack(plain.pack(codes), 112), codes)
+
+
+def test_every_kernel_waits_before_it_touches_memory():
+    """All kernels of these operators are launched so that they may begin while the launch in front still runs."""
+    csrc = os.path.join(ROOT, "llmini_b200", "csrc")
+    text = "".join(re.sub(r"//[^\n]*", "", open(os.path.join(csrc, n)).read()) for n in ("fp4_kernels.cu", "fp4_gemm_sm100.cu"))
+    kernels = re.findall(r"__global__[^;{]*?\b(k_fp4_\w+)\(([^{]*)\)\s*\{(.*?)\n\}", text, flags=re.S)
+    assert len(kernels) >= 7
+    for name, _, body in kernels:
+        assert body.count("stream_enter();") == 1, name
+        before = body.split("stream_enter();")[0]
+        assert "return" not in re.sub(r"\{ return [^}]*\}", "", before), name
+        assert "ld.global" not in before and "tma_load" not in before, name
+    for form in ("__ldg(", "ld.global.nc", "const float *__restrict__"):
+        assert form not in text, form

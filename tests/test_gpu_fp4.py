@@ -1,0 +1,559 @@
+"""The 4-bit operators against their definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import llmini_b200 as b2
+from tests import fp4_plain as plain
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+@pytest.fixture(scope="module")
+def module():
+    return b2.Nvfp4LinearModule()
+
+
+def activations(rng, rows, cols, dtype):
+    """Values with outlier columns, blocks of zeros, and many that lie exactly between two codes."""
+    x = rng.standard_normal((rows, cols))
+    x[:, rng.random(cols) < 0.02] *= 30
+    # multiples of the row maximum that are borders of the E2M1 grid times a power of two
+    ties = rng.random((rows, cols)) < 0.2
+    top = np.exp2(np.floor(np.log2(np.abs(x).max(1, keepdims=True))))
+    x = np.where(ties, top * rng.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], (rows, cols)) * np.exp2(rng.integers(-6, 1, (rows, cols))) / 8, x)
+    if cols > 40:
+        x[:, 16:32] = 0
+    return torch.from_numpy(x).float().to(TYPES[dtype])
+
+
+def check_operand(out, x64, whole=False):
+    codes, s, g = plain.quantise(x64, whole)
+    rows, k = codes.shape
+    assert (out.rows, out.k) == (rows, k)
+    got_g = out.scale.cpu().numpy().astype(np.float64)
+    np.testing.assert_array_equal(got_g, g[:1] if whole else g)
+    got_s, padding = plain.untiled(out.scales.cpu().numpy(), rows, k // 16)
+    np.testing.assert_array_equal(got_s, s)
+    assert not padding.any()
+    got = plain.unpack(out.bytes.cpu().numpy(), k)
+    # a code of zero may have either sign
+    np.testing.assert_array_equal(np.where(got == 8, 0, got), np.where(codes == 8, 0, codes))
+
+
+SHAPES = [(1, 16), (1, 1), (7, 17), (33, 1000), (130, 2048), (5, 2050), (129, 1600), (3, 8208), (2, 33000), (300, 64)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols", SHAPES)
+def test_quantize_rows(module, rows, cols, dtype):
+    x = activations(np.random.default_rng(rows * 7 + cols), rows, cols, dtype)
+    out = b2.Nvfp4Operand.empty(rows, cols)
+    out.scales.fill_(0x7f)   # padding behind the blocks of a row is written
+    module.quantize_rows(x.cuda(), out)
+    check_operand(out, plain.to_double(x))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (16, 1), (1, 130), (17, 7), (777, 100), (128, 128), (300, 1600), (1000, 33), (40, 2050)])
+def test_quantize_columns(module, rows, cols, dtype):
+    x = activations(np.random.default_rng(rows * 5 + cols), rows, cols, dtype)
+    out = b2.Nvfp4Operand.empty(cols, rows, per_row=False)
+    out.scales.fill_(0x7f)
+    module.quantize_columns(x.cuda(), out, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    check_operand(out, plain.to_double(x).T, whole=True)
+
+
+@pytest.mark.parametrize("offset,pad", [(0, 8), (1, 0), (1, 3), (4, 4), (8, 0)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantize_views(module, offset, pad, dtype):
+    """Rows with gaps and starts on every kind of boundary."""
+    rows, cols = 70, 200
+    x = activations(np.random.default_rng(3), rows, cols, dtype)
+    memory = torch.full((rows * (cols + pad) + offset,), float("nan"), dtype=x.dtype, device="cuda")
+    view = memory[offset:].view(rows, cols + pad)[:, :cols]
+    view.copy_(x)
+    out = b2.Nvfp4Operand.empty(rows, cols)
+    module.quantize_rows(view, out)
+    check_operand(out, plain.to_double(x))
+    out = b2.Nvfp4Operand.empty(cols, rows, per_row=False)
+    module.quantize_columns(view, out, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    check_operand(out, plain.to_double(x).T, whole=True)
+
+
+def test_rows_at_the_ends_of_the_range(module):
+    """Rows of zeros, of the type's smallest and largest values, and rows that are not finite."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((12, 70)).astype(np.float32)
+    x[0] = 0
+    x[1] *= np.float32(2.0 ** -126)
+    x[2] = np.float32(2.0 ** -149)
+    x[3] *= np.float32(2.0 ** 125)
+    x[4] = np.finfo(np.float32).max
+    x[5, 3] = np.inf
+    x[6, 69] = np.nan
+    x[7, 16:32] = -np.inf
+    x[8] *= np.float32(2.0 ** -101)
+    x[9] = -0.0
+    x[10, 1:] *= np.float32(2.0 ** -20)
+    out = b2.Nvfp4Operand.empty(12, 70)
+    module.quantize_rows(torch.from_numpy(x).cuda(), out)
+    check_operand(out, x)
+    columns = b2.Nvfp4Operand.empty(70, 12, per_row=False)
+    module.quantize_columns(torch.from_numpy(x).cuda(), columns, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    assert torch.isnan(columns.scale).all() and not columns.bytes[:, :8].any()
+    tame = x[[0, 1, 2, 8, 9]]
+    columns = b2.Nvfp4Operand.empty(70, 5, per_row=False)
+    module.quantize_columns(torch.from_numpy(tame).cuda(), columns, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    check_operand(columns, tame.T, whole=True)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,cols,whole", [(1, 1, False), (7, 100, False), (130, 1600, True), (3, 5000, False)])
+def test_decode_gives_the_values_that_codes_stand_for(module, rows, cols, whole, dtype):
+    rng = np.random.default_rng(rows)
+    k = -(-cols // 16) * 16
+    v, packed, s, g = plain.random_operand(rng, rows, k, not whole, -(-k // 32) * 16)
+    o = b2.Nvfp4Operand(torch.from_numpy(packed).cuda(), torch.from_numpy(plain.tiled(s)).cuda(), torch.from_numpy(g).cuda(), rows, k)
+    out = torch.full((rows, cols + 3), -7.0, dtype=TYPES[dtype], device="cuda")
+    module.decode(o, out[:, :cols])
+    got, want = plain.to_double(out), v[:, :cols]
+    assert (got[:, cols:] == -7).all()
+    # a product in FP32 and one rounding to the type (exact where g is a power of two and the value in range)
+    bound = np.abs(want) * (2.0 ** -24 + plain.half_step(TYPES[dtype])) * 1.001 + (2.0 ** -25 if dtype == "f16" else 0)
+    assert (np.abs(got[:, :cols] - want) <= bound).all()
+
+
+@pytest.mark.parametrize("layout", [b2.SCALES_CSF, b2.SCALES_RAW, b2.SCALES_SM100])
+def test_decode_reads_the_optimizers_weights(module, layout):
+    rows, k = 130, 384
+    x = torch.from_numpy(np.random.default_rng(1).standard_normal((rows, k)).astype(np.float32) * 0.02).cuda()
+    raw = b2.Nvfp4Tensor.empty(rows, k, b2.SCALES_RAW)
+    b2.Nvfp4QuantModule().fp32_to_nvfp4_four_six(x, x.abs().max().reshape(1), raw.bytes, raw.scales, raw.global_scale, rows * k // 16, b2.SCALES_RAW)
+    s = raw.scales.cpu().numpy().reshape(rows, -1)
+    t = raw
+    if layout == b2.SCALES_CSF:
+        t = b2.Nvfp4Tensor(raw.bytes, torch.from_numpy(b2.csf_encode_host(s.reshape(-1), rows, k)).cuda(), raw.global_scale, rows, k, layout)
+    elif layout == b2.SCALES_SM100:
+        t = b2.Nvfp4Tensor(raw.bytes, b2.scales_to_sm100(raw.scales, b2.SCALES_RAW, rows, k), raw.global_scale, rows, k, layout)
+    out = torch.empty(rows, k, device="cuda")
+    module.decode(t, out)
+    want = plain.values(plain.unpack(raw.bytes.cpu().numpy().reshape(rows, -1), k), s, raw.global_scale.item())
+    assert (np.abs(plain.to_double(out) - want) <= np.abs(want) * 2.0 ** -24).all()
+    # the quantiser's own error: half a step of the code grid (1, of values up to 6), and what saturates of a block scale rounded
+    # down by 2^-4
+    step = np.repeat(plain.e4m3_grid()[s] * raw.global_scale.item(), 16, 1)
+    assert (np.abs(plain.to_double(out) - plain.to_double(x)) <= 1.001 * step).all()
+
+
+# ---- the product ------------------------------------------------------------------------------------------------------------
+def operand(rng, rows, k, per_row, spare=0):
+    """(values, Nvfp4Operand) with `spare` bytes behind every row, which are not the product's to read."""
+    v, packed, s, g = plain.random_operand(rng, rows, k, per_row, -(-k // 32) * 16 + spare)
+    packed[:, k // 2:] = 0x77
+    t = plain.tiled(s)
+    o = b2.Nvfp4Operand(torch.from_numpy(packed).cuda(), torch.from_numpy(t).cuda(), torch.from_numpy(g).cuda(), rows, k)
+    return v, o
+
+
+def product_bound(a, b, want, dtype):
+    """FP32 sums: every addition of a product is off by at most 2^-23 of what has been added up by then (a truncated sum), scaling
+    and bias by 2^-24 each; then half a step of the type."""
+    terms = np.abs(a) @ np.abs(b).T
+    return terms * (a.shape[1] * 2.0 ** -23 + 2.0 ** -22) + np.abs(want) * (2.0 ** -22 + plain.half_step(dtype)) + (2.0 ** -25 if dtype == torch.float16 else 0)
+
+
+PRODUCTS = [(1, 1, 16), (1, 4800, 1600), (3, 40, 48), (16, 128, 256), (24, 1600, 6400), (33, 257, 64), (64, 1000, 320), (65, 300, 96), (127, 129, 784),
+            (128, 128, 64), (129, 127, 1616), (200, 1000, 512), (257, 511, 1040), (777, 1600, 1600), (1000, 2304, 768), (300, 5025, 160),
+            (2048, 2304, 768), (2100, 4000, 400)]
+
+
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_matmul(module, m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    a, oa = operand(rng, m, k, True)
+    b, ob = operand(rng, n, k, False, 16)
+    want = a @ b.T
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+        module.matmul(oa, ob, out)
+        assert module.status() == 0
+        err = np.abs(plain.to_double(out) - want)
+        assert (err <= product_bound(a, b, want, dtype)).all(), (dtype, np.argwhere(~(err <= product_bound(a, b, want, dtype)))[:5])
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (0, 3), (8, 8)])
+def test_matmul_epilogue(module, m, n, k, dtype, offset, pad):
+    """Scales for rows of both sides, a bias, rows of c with gaps and starts on every boundary: nothing else of c's memory changes."""
+    rng = np.random.default_rng(m * n)
+    a, oa = operand(rng, m, k, True)
+    b, ob = operand(rng, n, k, True)
+    a, b = a / 64, b / 64
+    oa.scale /= 64
+    ob.scale /= 64
+    bias = rng.standard_normal(n).astype(np.float32)
+    memory = torch.full((offset + m * (n + pad) + 64,), -3.0, dtype=TYPES[dtype], device="cuda")
+    c = memory[offset:offset + m * (n + pad)].view(m, n + pad)[:, :n]
+    module.matmul(oa, ob, c, bias=torch.from_numpy(bias).cuda())
+    want = a @ b.T + bias.astype(np.float64)
+    assert (np.abs(plain.to_double(c) - want) <= product_bound(a, b, want, TYPES[dtype]) + np.abs(bias) * 2.0 ** -22).all()
+    c.fill_(-3.0)
+    assert (memory == -3.0).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512)])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_matmul_accumulates(module, m, n, k, pad):
+    rng = np.random.default_rng(m + 1)
+    a, oa = operand(rng, m, k, False)
+    b, ob = operand(rng, n, k, False)
+    start = rng.standard_normal((m, n + pad)).astype(np.float32)
+    c = torch.from_numpy(start).cuda()
+    module.matmul(oa, ob, c[:, :n], accumulate=True)
+    want = a @ b.T + start[:, :n]
+    assert (np.abs(plain.to_double(c)[:, :n] - want) <= product_bound(a, b, want, torch.float32) + np.abs(start[:, :n]) * 2.0 ** -22).all()
+    assert (plain.to_double(c)[:, n:] == start[:, n:]).all()
+
+
+def test_matmul_keeps_rows_apart(module):
+    """A row that is not finite makes its own results NaN and no others; scales behind the last row of an operand do not matter."""
+    rng = np.random.default_rng(9)
+    for m, n in ((40, 300), (300, 500)):
+        a, oa = operand(rng, m, 160, True)
+        b, ob = operand(rng, n, 160, False)
+        for o, rows in ((oa, m), (ob, n)):
+            full = o.scales.view(-(-rows // 128), 3, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-1, 12).clone()
+            full[rows:] = 0x7f
+            o.scales.copy_(full.view(-1, 4, 32, 3, 4).permute(0, 3, 2, 1, 4).reshape(-1))
+        oa.scale[7] = float("nan")
+        out = torch.empty(m, n, device="cuda")
+        module.matmul(oa, ob, out)
+        want = a @ b.T
+        bad = np.arange(m) == 7
+        got = plain.to_double(out)
+        assert np.isnan(got[bad]).all()
+        assert (np.abs(got - want)[~bad] <= product_bound(a, b, want, torch.float32)[~bad]).all()
+
+
+def test_matmul_does_not_depend_on_the_launch(module):
+    """The same bits again, and on another stream."""
+    rng = np.random.default_rng(2)
+    for m, n, k in ((1, 4800, 1600), (24, 1600, 6400), (600, 1000, 512), (2100, 4000, 400)):
+        _, oa = operand(rng, m, k, True)
+        _, ob = operand(rng, n, k, False)
+        outs = [torch.empty(m, n, device="cuda") for _ in range(3)]
+        module.matmul(oa, ob, outs[0])
+        module.matmul(oa, ob, outs[1])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            module.matmul(oa, ob, outs[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+# ---- the linear layer ---------------------------------------------------------------------------------------------------------
+def rounded(x, whole=False):
+    codes, s, g = plain.quantise(x, whole)
+    return plain.values(codes, s, g)[:, : x.shape[1]]
+
+
+def within(got, a, b, dtype, extra=0.0):
+    """got = a b^T (+ extra) to the product's bound"""
+    want = a @ b.T + extra
+    assert (np.abs(plain.to_double(got) - want) <= product_bound(a, b, want, dtype) + np.abs(extra) * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1, 64, 40), (1, 1600, 4800), (7, 96, 33), (24, 6400, 1600), (200, 768, 1000), (1030, 160, 300)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_linear_forward(module, tokens, inputs, outputs, dtype):
+    rng = np.random.default_rng(tokens + outputs)
+    x = activations(rng, tokens, inputs, dtype) / 64
+    w, ow = operand(rng, outputs, inputs, False)
+    bias = rng.standard_normal(outputs).astype(np.float32)
+    out = torch.empty(tokens, outputs, dtype=TYPES[dtype], device="cuda")
+    module.linear_forward(x.cuda(), ow, out, b2.Nvfp4LinearScratch(tokens, inputs, outputs), bias=torch.from_numpy(bias).cuda())
+    within(out, rounded(plain.to_double(x)), w, TYPES[dtype], bias.astype(np.float64))
+
+
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1, 16, 16), (7, 100, 33), (130, 272, 496), (777, 160, 320), (300, 1000, 770)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_linear_backward(module, tokens, inputs, outputs, dtype):
+    rng = np.random.default_rng(tokens + outputs)
+    x, grad = activations(rng, tokens, inputs, dtype), activations(rng, tokens, outputs, dtype) / 64
+    x64, grad64 = plain.to_double(x), plain.to_double(grad)
+    wt, owt = operand(rng, inputs, -(-outputs // 16) * 16, False)
+    args = dict(device="cuda", dtype=TYPES[dtype])
+    scratch = b2.Nvfp4LinearScratch(tokens, inputs, outputs, backward=True)
+    k = wt.shape[1]
+    gr = np.zeros((tokens, k))
+    gr[:, :outputs] = rounded(grad64)
+    gc, xc = rounded(grad64.T, True), rounded(x64.T, True)
+    for want_x, want_w, accumulate in ((True, True, False), (True, False, False), (False, True, False), (True, True, True)):
+        start = rng.standard_normal((outputs, inputs)).astype(np.float32)
+        grad_x = torch.full((tokens, inputs), -3.0, **args) if want_x else None
+        grad_w = torch.from_numpy(start).cuda() if want_w else None
+        module.linear_backward(grad.cuda(), x.cuda(), owt, grad_x, grad_w, scratch, accumulate=accumulate)
+        if want_x:
+            within(grad_x, gr, wt, TYPES[dtype])
+        if want_w:
+            within(grad_w, gc, xc, torch.float32, start.astype(np.float64) if accumulate else 0.0)
+
+
+def test_linear_gradients_are_those_of_the_layer(module):
+    """Against differences of sum(grad * (x W^T)): the gradients are off by what the rounding of their operands to 4 bits is.  A
+    block's values are off by half a step of E2M1, 1/2 of values 4 .. 6 down to 1/4 of those below 2, in units of max / 6; normal
+    values by 0.10 of their size together.  Three sigma above the two operands' 0.14, for sums over 256 or more."""
+    rng = np.random.default_rng(4)
+    tokens, inputs, outputs = 256, 320, 384
+    x, grad, w = (torch.from_numpy(rng.standard_normal(s).astype(np.float32)).cuda() for s in ((tokens, inputs), (tokens, outputs), (outputs, inputs)))
+    owt = b2.Nvfp4Operand.empty(inputs, outputs, per_row=False)
+    module.quantize_columns(w, owt, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    grad_x, grad_w = torch.empty_like(x), torch.empty_like(w)
+    module.linear_backward(grad, x, owt, grad_x, grad_w, b2.Nvfp4LinearScratch(tokens, inputs, outputs, backward=True))
+    loss = lambda x, w: (grad.double() * (x.double() @ w.double().T)).sum()
+    for got, at, other in ((grad_x, x, 0), (grad_w, w, 1)):
+        for _ in range(4):
+            d = torch.randn(at.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(_)) * 0.5
+            ends = [loss(*((at + s * d, w) if other == 0 else (x, at + s * d))) for s in (1, -1)]
+            slope = ((ends[0] - ends[1]) / 2).item()
+            scale = (torch.linalg.vector_norm((grad.double() @ w.double() if other == 0 else grad.double().T @ x.double())) * torch.linalg.vector_norm(d.double()) / d.numel() ** 0.5).item()
+            assert abs((got.double() * d.double()).sum().item() - slope) <= 3 * 0.15 * scale
+
+
+def test_linear_backward_of_no_tokens(module):
+    w = torch.full((40, 24), 5.0, device="cuda")
+    s = b2.Nvfp4LinearScratch(0, 24, 40, backward=True)
+    x, grad = torch.empty(0, 24, device="cuda"), torch.empty(0, 40, device="cuda")
+    module.linear_backward(grad, x, None, None, w, s, accumulate=True)
+    assert (w == 5).all()
+    module.linear_backward(grad, x, None, None, w, s)
+    assert (w == 0).all()
+
+
+def test_a_training_step_together(module):
+    """The optimizer's weights through the layer and back: a plan that leaves its scales in SCALES_SM100, forward, backward from
+    the quantised transpose of the masters, the weight gradient added up over two micro-batches into the plan's gradient buffer,
+    and the next optimizer step on it; then the same as a captured graph."""
+    from tests.gpu_util import host
+    rng = np.random.default_rng(8)
+    tokens, inputs, outputs = 96, 256, 384
+    slot = b2.MuonSlot.allocate(outputs, inputs, scale_layout=b2.SCALES_SM100)
+    master = torch.from_numpy(rng.standard_normal((outputs, inputs)).astype(np.float32) * 0.02).cuda()
+    slot.z_master.copy_(master.view_as(slot.z_master))
+    slot.x_master.copy_(master.view_as(slot.x_master))
+    slot.grad.copy_(torch.from_numpy(rng.standard_normal((outputs, inputs)).astype(np.float32) * 1e-3).view_as(slot.grad))
+    plan = b2.MuonPlan([(outputs, inputs)], scale_layout=b2.SCALES_SM100)
+    opt, table, step = b2.OptimizerModule(), b2.slot_table([slot]), b2.MuonMegaUpdateArgs(learning_rate=0.02)
+    opt.muon_mega_update(plan, table, step)
+    weight = b2.Nvfp4Operand(slot.bytes.view(outputs, inputs // 2), slot.scales, slot.global_scale, outputs, inputs)
+    weight_t = b2.Nvfp4Operand.empty(inputs, outputs, per_row=False)
+    maxima = torch.empty(b2.NVFP4_MAXIMA, device="cuda")
+    x = [torch.randn(tokens, inputs, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    grad = [torch.randn(tokens, outputs, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    y, grad_x = torch.empty(tokens, outputs, device="cuda", dtype=torch.bfloat16), torch.empty(tokens, inputs, device="cuda", dtype=torch.bfloat16)
+    forward, backward = b2.Nvfp4LinearScratch(tokens, inputs, outputs), b2.Nvfp4LinearScratch(tokens, inputs, outputs, backward=True)
+    grad_w = slot.grad.view(outputs, inputs)
+
+    def layer():
+        module.quantize_columns(slot.x_master.view(outputs, inputs), weight_t, maxima)
+        for i in range(2):
+            module.linear_forward(x[i], weight, y, forward)
+            module.linear_backward(grad[i], x[i], weight_t, grad_x, grad_w, backward, accumulate=i > 0)
+
+    layer()
+    torch.cuda.synchronize()
+    w64 = plain.values(plain.unpack(host(weight.bytes), inputs), plain.untiled(host(slot.scales), outputs, inputs // 16)[0], slot.global_scale.item())
+    wt64 = rounded(plain.to_double(slot.x_master.view(outputs, inputs)).T, True)
+    within(y, rounded(plain.to_double(x[1])), w64, torch.bfloat16)
+    within(grad_x, rounded(plain.to_double(grad[1])), wt64, torch.bfloat16)
+    sides = [(rounded(plain.to_double(grad[i]).T, True), rounded(plain.to_double(x[i]).T, True)) for i in range(2)]
+    want = sum(g @ xx.T for g, xx in sides)
+    assert (np.abs(plain.to_double(grad_w) - want) <= sum(product_bound(g, xx, want, torch.float32) for g, xx in sides)).all()
+    eager = [t.clone() for t in (y, grad_x, grad_w)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer()
+    for t in (y, grad_x, grad_w):
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(eager, (y, grad_x, grad_w)))
+    for t in x + grad:
+        t.mul_(2.0)   # the graph reads its inputs anew; scales are powers of two, so everything is exactly twice (four times) as large
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, 2 * eager[0]) and torch.equal(grad_x, 2 * eager[1]) and torch.equal(grad_w, 4 * eager[2])
+    before = slot.x_master.clone()
+    opt.muon_mega_update(plan, table, step)
+    assert plan.status() == 0 and module.status() == 0
+    assert torch.isfinite(slot.x_master).all() and not torch.equal(before, slot.x_master)
+    plan.close()
+
+
+# ---- the cache ------------------------------------------------------------------------------------------------------------------
+def cache_values(side, dim):
+    """[pages, page_size, heads, dim] values of one side of a cache, in 64 bits."""
+    codes, s, e = (t.cpu().numpy() for t in side)
+    n = int(np.prod(e.shape))
+    g = np.where(e.reshape(-1) == 255, np.nan, np.exp2(e.reshape(-1).astype(np.float64) - 127))
+    return plain.values(plain.unpack(codes.reshape(n, -1), dim), s.reshape(n, -1), g).reshape(*e.shape, dim)
+
+
+@pytest.mark.parametrize("heads,dim,value_dim,page", [(1, 16, 16, 1), (4, 64, 64, 16), (25, 64, 64, 32), (3, 96, 128, 7), (2, 576, 512, 64), (1, 1024, 16, 5)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_cache(module, heads, dim, value_dim, page, dtype):
+    """Tokens written to scattered slots out of a fused projection, some left out; sequences of every length read back."""
+    rng = np.random.default_rng(dim + page)
+    pages, sequences, width = 40, 6, 6
+    longest = width * page + 3
+    cache = b2.Nvfp4PagedCache.empty(pages, page, heads, dim, value_dim)
+    for side in (cache.key, cache.value):
+        for t in side:
+            t.random_(0, 120)
+    before = [t.clone() for side in (cache.key, cache.value) for t in side]
+    tokens = min(pages * page, 50)
+    slots = rng.permutation(pages * page)[:tokens].astype(np.int64)
+    leave = [0, tokens // 2] if tokens > 4 else []
+    for i, bad in zip(leave, (-1, pages * page)):
+        slots[i] = bad
+    fused = activations(rng, tokens, heads * (dim + value_dim) + 8, dtype).cuda()
+    if tokens > 3:
+        fused[3, 1] = float("inf")   # one vector
+    key = fused[:, : heads * dim].unflatten(1, (heads, dim))
+    value = fused[:, heads * dim: heads * (dim + value_dim)].unflatten(1, (heads, value_dim))
+    module.cache_write(cache, torch.from_numpy(slots).cuda(), key, value)
+    kept = np.ones(pages * page, bool)
+    for i, slot in enumerate(slots):
+        if 0 <= slot < pages * page:
+            kept[slot] = False
+    for j, (side, new, d) in enumerate(((cache.key, key, dim), (cache.value, value, value_dim))):
+        codes, s, g = plain.quantise(plain.to_double(new).reshape(-1, d))
+        got = cache_values(side, d).reshape(pages * page, heads, d)
+        want = plain.values(codes, s, g).reshape(tokens, heads, d)
+        for i, slot in enumerate(slots):
+            if 0 <= slot < pages * page:
+                np.testing.assert_array_equal(got[slot], want[i])
+        for t, old in zip(side, before[3 * j: 3 * j + 3]):   # slots that no token went to
+            assert torch.equal(t.view(pages * page, -1)[torch.from_numpy(kept)], old.view(pages * page, -1)[torch.from_numpy(kept)])
+    # the old slots of random bytes hold numbers too
+    table = rng.integers(0, pages, (sequences, width)).astype(np.int32)
+    table[1, 0], table[2, width - 1] = -1, pages
+    lengths = np.array([width * page, 1, width * page + 2, 0, -5, page], np.int32)
+    outs = [torch.full((sequences, longest, heads, d + 8), -3.0, dtype=TYPES[dtype], device="cuda")[..., :d] for d in (dim, value_dim)]
+    module.cache_read(cache, torch.from_numpy(table).cuda(), torch.from_numpy(lengths).cuda(), *outs)
+    for side, out, d in ((cache.key, outs[0], dim), (cache.value, outs[1], value_dim)):
+        v = cache_values(side, d)
+        got = plain.to_double(out)
+        for b in range(sequences):
+            n = int(np.clip(lengths[b], 0, width * page))
+            for t in range(n):
+                p = table[b, t // page]
+                want = v[p, t % page] if 0 <= p < pages else np.full((heads, d), np.nan)
+                want = torch.from_numpy(want).to(TYPES[dtype]).double().numpy()
+                np.testing.assert_array_equal(got[b, t], want)
+            assert (got[b, n:] == -3).all()
+        assert (out._base[..., d:] == -3).all()
+
+
+def test_cache_beyond_32_bits(module):
+    """A cache of more than 2^32 bytes of codes: the last page's, and the same tokens' near the start."""
+    pages, page, heads, dim = 33000, 64, 16, 256
+    codes = torch.empty(pages, page, heads, dim // 2, dtype=torch.uint8, device="cuda")
+    cache = b2.Nvfp4PagedCache((codes, torch.empty(pages, page, heads, dim // 16, dtype=torch.uint8, device="cuda"),
+                                torch.empty(pages, page, heads, dtype=torch.uint8, device="cuda")))
+    assert codes.numel() > 1 << 32
+    key = torch.randn(2 * page, heads, dim, device="cuda", dtype=torch.bfloat16)
+    place = torch.arange(page, device="cuda")
+    module.cache_write(cache, torch.cat([place + page, place + (pages - 1) * page]), key)
+    out = torch.zeros(2, page, heads, dim, device="cuda", dtype=torch.bfloat16)
+    module.cache_read(cache, torch.tensor([[1], [pages - 1]], dtype=torch.int32, device="cuda"), torch.full((2,), page, dtype=torch.int32, device="cuda"), out)
+    want = rounded(plain.to_double(key).reshape(-1, dim)).reshape(2, page, heads, dim)
+    np.testing.assert_array_equal(plain.to_double(out), torch.from_numpy(want).bfloat16().double().numpy())
+
+
+def test_tensors_beyond_32_bits(module):
+    """More than 2^32 values: the last rows come out as they do by themselves."""
+    rows, cols = 66000, 65600
+    x = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16)
+    x[:256].normal_()
+    for r in range(256, rows, 256):
+        x[r:r + 256] = x[:min(256, rows - r)]
+    x[-1].mul_(3.0)
+    big = b2.Nvfp4Operand.empty(rows, cols)
+    module.quantize_rows(x, big)
+    tail = b2.Nvfp4Operand.empty(5, cols)
+    module.quantize_rows(x[-5:].clone(), tail)
+    assert torch.equal(big.bytes[-5:, : cols // 2], tail.bytes[:, : cols // 2]) and torch.equal(big.scale[-5:], tail.scale)
+    back, part = torch.empty_like(x), torch.empty(5, cols, device="cuda", dtype=torch.bfloat16)
+    module.decode(big, back)
+    module.decode(tail, part)
+    assert torch.equal(back[-5:], part)
+    del back, big
+    columns = b2.Nvfp4Operand.empty(cols, rows, per_row=False)
+    module.quantize_columns(x, columns, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    some = b2.Nvfp4Operand.empty(16, rows, per_row=False)
+    module.quantize_columns(torch.cat([x[:, -15:], torch.full((rows, 1), x.abs().max().item(), device="cuda", dtype=x.dtype)], 1), some,
+                            torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+    assert torch.equal(columns.bytes[-15:, : rows // 2], some.bytes[:15, : rows // 2]) and torch.equal(columns.scale, some.scale)
+    del columns, some
+    rng = np.random.default_rng(0)
+    a, oa = operand(rng, rows, 64, True)
+    b, ob = operand(rng, cols, 64, False)
+    module.matmul(oa, ob, x)
+    want = a[-300:] @ b[-300:].T
+    assert (np.abs(plain.to_double(x[-300:, -300:]) - want) <= product_bound(a[-300:], b[-300:], want, torch.bfloat16)).all()
+
+
+# ---- what is refused --------------------------------------------------------------------------------------------------------------
+def test_refusals(module):
+    f = lambda *s, dtype=torch.float32, device="cuda": torch.zeros(*s, dtype=dtype, device=device)
+    o = b2.Nvfp4Operand.empty
+    with pytest.raises(ValueError):
+        module.quantize_rows(f(4, 32, device="cpu"), o(4, 32))
+    with pytest.raises(ValueError):
+        module.quantize_rows(f(4, 32, dtype=torch.float64), o(4, 32))
+    with pytest.raises(ValueError):
+        module.quantize_rows(f(32, 4).T, o(4, 32))
+    with pytest.raises(ValueError):
+        module.quantize_rows(f(1, 32).expand(4, 32), o(4, 32))
+    for x, out in ((f(4, 32), o(5, 32)), (f(4, 32), o(4, 48)), (f(4, 32), o(4, 32, per_row=False))):
+        with pytest.raises(b2.B2Error):
+            module.quantize_rows(x, out)
+    with pytest.raises(ValueError):
+        module.quantize_columns(f(4, 32), o(32, 4, per_row=False), f(10))
+    with pytest.raises(b2.B2Error):
+        module.quantize_columns(f(4, 32), o(4, 32, per_row=False), f(1024))
+    for a, b, c in ((o(4, 32), o(5, 48), f(4, 5)), (o(4, 32), o(5, 32), f(5, 4)), (o(4, 32), o(5, 32), f(4, 6))):
+        with pytest.raises(b2.B2Error):
+            module.matmul(a, b, c)
+    with pytest.raises(b2.B2Error):
+        module.matmul(o(4, 32), o(5, 32), f(4, 5, dtype=torch.bfloat16), accumulate=True)
+    with pytest.raises(ValueError):
+        module.matmul(o(4, 32), o(5, 32), f(4, 5), bias=f(4))
+    with pytest.raises(ValueError):
+        module.linear_forward(f(4, 32), o(5, 32), f(4, 5), b2.Nvfp4LinearScratch(4, 32, 5, backward=True))
+    with pytest.raises(ValueError):
+        b2.Nvfp4Operand(f(4, 8, dtype=torch.uint8), f(512, dtype=torch.uint8), f(4), 4, 16)   # rows on 8-byte boundaries
+    with pytest.raises(ValueError):
+        b2.Nvfp4Operand(f(4, 16, dtype=torch.uint8), f(100, dtype=torch.uint8), f(4), 4, 32)  # too few scales
+    cache = b2.Nvfp4PagedCache.empty(4, 2, 3, 32)
+    slots = torch.zeros(5, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        module.cache_write(cache, slots, f(5, 3, 32))
+    with pytest.raises(ValueError):
+        module.cache_write(cache, slots, f(5, 3, 48), f(5, 3, 48))
+    with pytest.raises(ValueError):
+        module.cache_write(cache, slots.int(), f(5, 3, 32), f(5, 3, 32))
+    with pytest.raises(ValueError):
+        module.cache_write(cache, slots, f(5, 3, 32), f(5, 3, 32, dtype=torch.bfloat16))
+    with pytest.raises(b2.B2Error):
+        b2.Nvfp4LinearModule().cache_write(b2.Nvfp4PagedCache.empty(4, 2, 3, 1040), slots, f(5, 3, 1040), f(5, 3, 1040))
+    # nothing to do is no error
+    module.quantize_rows(f(0, 32), o(0, 32))
+    module.matmul(o(0, 32), o(5, 32), f(0, 5))
+    module.matmul(o(4, 32), o(0, 32, per_row=False), f(4, 0))
+    module.cache_write(cache, slots[:0], f(0, 3, 32), f(0, 3, 32))

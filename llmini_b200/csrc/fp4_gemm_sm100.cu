@@ -6,6 +6,7 @@
 // four MMAs.  The block scales of 128 rows and 64 values of K are a 512-byte tile, stored as the copy wants it.
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include <cuda.h>
 
@@ -19,6 +20,7 @@ namespace {
 
 constexpr uint32_t kStageK = 256;       // values of K in a pipeline stage
 constexpr uint32_t kScaleTile = 512;    // bytes: 128 rows x 64 values of K
+constexpr uint32_t kSlabs = 1, kSlabBytes = kSlabs * 32 * 128;   // an epilogue warp's: 32 rows x 128 bytes of c each
 constexpr uint32_t kScaleBand = kStageK / 64 * kScaleTile;   // a stage's scales of 128 rows
 
 // Set when a bounded wait ran out (b2_nvfp4_status).
@@ -67,59 +69,71 @@ struct Epilogue {
     uint32_t a_rows, b_rows;   // a scale for every row of A (B)
     uint32_t type;             // of c
     uint32_t accumulate;
-    uint32_t vec;              // rows of c start on 32-byte boundaries
+    uint32_t bulk;             // rows of c start on 16-byte boundaries: c has a tensor map
+    uint32_t bias_vec;         // the bias on a 16-byte one
 };
 
-// 32 columns from `col` on of row `row`, `acc` their sums: scaled, biased, rounded, stored.
-__device__ __forceinline__ void store_columns(const Epilogue &e, uint32_t row, uint32_t col, const uint32_t *acc, float sa) {
-    if (row >= e.M || col >= e.N) return;
-    float v[32];
-    const float sb = e.b_rows ? 1.0f : *e.scale_b;
-    const float s = sa * sb;
+// Sums of 32 columns from `col` on, scaled (s: the scale of A's row, and B's where it has one for all) and biased.  `n` are there.
+__device__ __forceinline__ void finish_columns(const Epilogue &e, uint32_t col, uint32_t n, const uint32_t *acc, float s, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]) * s;
-    const uint32_t n = min(e.N - col, 32u);
     if (e.b_rows) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
             if ((uint32_t)i < n) v[i] *= e.scale_b[col + i];
     }
     if (e.bias) {
+        if (n == 32 && e.bias_vec) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if ((uint32_t)i < n) v[i] += e.bias[col + i];
-    }
-    if (e.type == B2_TYPE_F32) {
-        float *p = reinterpret_cast<float *>(e.c + (uint64_t)row * e.pitch) + col;
-        if (n == 32 && e.vec) {
-            if (e.accumulate) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 o = reinterpret_cast<const float4 *>(p)[i];
-                    v[4 * i] += o.x; v[4 * i + 1] += o.y; v[4 * i + 2] += o.z; v[4 * i + 3] += o.w;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float4 o = reinterpret_cast<const float4 *>(e.bias + col)[i];
+                v[4 * i] += o.x; v[4 * i + 1] += o.y; v[4 * i + 2] += o.z; v[4 * i + 3] += o.w;
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st_global_32(p + 8 * i, reinterpret_cast<const uint32_t *>(v) + 8 * i);
         } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-                if ((uint32_t)i < n) p[i] = e.accumulate ? p[i] + v[i] : v[i];
-        }
-    } else {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pack_operands(v[2 * i], v[2 * i + 1], e.type == B2_TYPE_F16);
-        uint16_t *p = reinterpret_cast<uint16_t *>(e.c + (uint64_t)row * e.pitch) + col;
-        if (n == 32 && e.vec) {
-            st_global_32(p, w);
-            st_global_32(p + 16, w + 8);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if ((uint32_t)i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+                if ((uint32_t)i < n) v[i] += e.bias[col + i];
         }
     }
+}
+__device__ __forceinline__ void st_shared_16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void store_value(const Epilogue &e, uint32_t row, uint32_t col, float v) {
+    uint8_t *line = e.c + (uint64_t)row * e.pitch;
+    if (e.type == B2_TYPE_F32) {
+        float *p = reinterpret_cast<float *>(line) + col;
+        *p = e.accumulate ? *p + v : v;
+    } else {
+        reinterpret_cast<uint16_t *>(line)[col] = (uint16_t)(e.type == B2_TYPE_F16 ? f32_to_f16_bits(v) : f32_to_bf16_bits(v));
+    }
+}
+// The old values of 32 columns that are all there, of a row on a 16-byte boundary.
+__device__ __forceinline__ void add_old(const Epilogue &e, uint32_t row, uint32_t col, float (&v)[32]) {
+    const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(e.c + (uint64_t)row * e.pitch) + col);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 o = p[i];
+        v[4 * i] += o.x; v[4 * i + 1] += o.y; v[4 * i + 2] += o.z; v[4 * i + 3] += o.w;
+    }
+}
+__device__ __forceinline__ void tma_store_2d(uint64_t map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// Where rows of c start on any boundary: through `slab` (32 x 32 floats of this warp, a row's columns in an order of its own), so
+// that a store instruction of the warp writes neighbouring values of a row and not one value of each of 32 rows.
+__device__ __forceinline__ void store_through(const Epilogue &e, uint32_t row0, uint32_t col, const float (&v)[32], float *slab) {
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (uint32_t i = 0; i < 32; ++i) slab[lane * 32 + (i ^ lane)] = v[i];
+    __syncwarp();
+    const uint32_t rows = min(32u, e.M - row0);
+    if (col + lane < e.N) {
+#pragma unroll 8
+        for (uint32_t r = 0; r < rows; ++r) store_value(e, row0 + r, col + lane, slab[r * 32 + (lane ^ r)]);
+    }
+    __syncwarp();
 }
 
 // Tile of a CTA (128 x BN), or of a pair of CTAs (256 x BN): each holds 128 rows of A, half of the rows of B and all of B's scales.
@@ -142,16 +156,18 @@ struct FCfg {
     // warps: producers of A, of B and of the scales, the MMA issuer, eight epilogue warps
     static constexpr int kProducerA = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 8, kProducerB = 10, kProducerS = 11;
     static constexpr int kThreads = 12 * 32;
-    static constexpr uint32_t kControl = 256;
-    static constexpr uint32_t kMaxStages = ((uint32_t)kSmemLimit - kControl - 1024) / kStageBytes;
+    static constexpr uint32_t kControl = 1024;
+    static constexpr uint32_t kBesides = kControl + kEpiWarps * kSlabBytes + 1024;   // (the slabs start on a 1024-byte boundary)
+    static constexpr uint32_t kMaxStages = ((uint32_t)kSmemLimit - kBesides) / kStageBytes;
     static constexpr uint32_t kStages = kMaxStages < 6 ? kMaxStages : 6;
-    static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kControl + 1024;
+    static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kBesides;
 };
 
 template <bool PAIR, int BN>
 __global__ void __launch_bounds__((FCfg<PAIR, BN>::kThreads), 1)
 k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
-           const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ Epilogue epi, uint32_t K, uint32_t tiles_m, uint32_t tiles) {
+           const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Epilogue epi,
+           uint32_t K, uint32_t tiles_m, uint32_t tiles) {
     using C = FCfg<PAIR, BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -253,16 +269,27 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                     const uint64_t ad = desc0 + stage * (C::kStageBytes >> 4), bd = ad + (C::kABytes >> 4);
                     const uint64_t sd = sdesc0 + ((stage * C::kStageBytes + C::kSfa) >> 4);
                     if (elect_one()) {
-                        const uint32_t steps = min(4u, (K - kb * kStageK + 63u) / 64u);
-                        for (uint32_t j = 0; j < steps; ++j) {
+                        // straight-line code: what bounds a stage is how fast one thread issues its sixteen instructions
+                        auto copy = [&](uint32_t j) {
                             tc_copy_scales<PAIR>(tmem + C::kSfaCol + 4 * j, sd + j * (kScaleTile >> 4));
 #pragma unroll
                             for (uint32_t b = 0; b < C::kBands; ++b)
                                 tc_copy_scales<PAIR>(tmem + C::kSfbCol + 4 * (j * C::kBands + b), sd + (((1 + b) * kScaleBand + j * kScaleTile) >> 4));
-                        }
-                        for (uint32_t j = 0; j < steps; ++j)
+                        };
+                        auto mma = [&](uint32_t j) {
                             tc_mma_fp4<PAIR>(d_tmem, ad + 2 * j, bd + 2 * j, idesc, tmem + C::kSfaCol + 4 * j, tmem + C::kSfbCol + 4 * j * C::kBands,
                                              kb != 0 || j != 0 ? 1u : 0u);
+                        };
+                        const uint32_t steps = min(4u, (K - kb * kStageK + 63u) / 64u);
+                        if (steps == 4) {
+                            copy(0); copy(1); copy(2); copy(3);
+                            mma(0); mma(1); mma(2); mma(3);
+                        } else {
+                            for (uint32_t j = 0; j < steps; ++j) {
+                                copy(j);
+                                mma(j);
+                            }
+                        }
                         tc_commit<PAIR>(empty_bar(stage));
                         if (kb + 1 == stages) tc_commit<PAIR>(tfull_bar(it & 1u));
                     }
@@ -272,37 +299,81 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
             }
         }
     } else {
-        // Warp w reads tensor-memory lanes 32 (w % 4) .. +31, and every other unit of 32 columns.
+        // Warp w reads tensor-memory lanes 32 (w % 4) .. +31, and every other unit of 64 columns.  Results go through slabs in
+        // shared memory (32 rows x 128 bytes) to bulk stores of whole lines.
         const uint32_t q = warp & 3, half = (warp - C::kEpiWarp0) >> 2;
         const uint32_t tempty_leader = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
-        constexpr uint32_t kUnits = BN / 32;
+        uint8_t *slabs = smem + C::kStages * C::kStageBytes + C::kControl + (warp - C::kEpiWarp0) * kSlabBytes;
+        uint32_t turn = 0;
+        const float sb = epi.b_rows ? 1.0f : *epi.scale_b;
         uint32_t it = 0;
         for (uint32_t t = first; t < tiles; t += stride, ++it) {
             const uint32_t tile_m = t % tiles_m, tile_n = t / tiles_m;
-            const uint32_t row = tile_m * C::kTileM + rank * 128 + 32 * q + lane;
-            const float sa = row < epi.M ? epi.scale_a[epi.a_rows ? row : 0] : 0.0f;
+            const uint32_t row0 = tile_m * C::kTileM + rank * 128 + 32 * q, row = row0 + lane;
+            const float s = row < epi.M ? epi.scale_a[epi.a_rows ? row : 0] * sb : 0.0f;
             const uint32_t n = mma_n(tile_n);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(it & 1u), (it >> 1) & 1u, abort_flag))) break;
             tc_fence_after();
             const uint32_t acc = tmem_base + (it & 1u) * C::kAcc1 + ((32u * q) << 16);
 #pragma unroll 1
-            for (uint32_t i = 0; i < kUnits / 2; ++i) {
+            for (uint32_t i = 0; i < BN / 128; ++i) {
                 // where the accumulators share columns, these first: the last ones of the first, the first ones of the second
-                const uint32_t p = 2 * i + half, unit = C::kShared && (it & 1u) == 0 ? kUnits - 1 - p : p;
-                uint32_t r[32];
-                const bool there = unit * 32 < n;
-                if (there) {
-                    tc_ld32(acc + unit * 32, r);
+                const uint32_t p = 2 * i + half, unit = C::kShared && (it & 1u) == 0 ? BN / 64 - 1 - p : p;
+                const uint32_t col0 = tile_n * BN + unit * 64;
+                uint32_t r[2][32];
+                if (unit * 64 < n) {
+                    tc_ld32(acc + unit * 64, r[0]);
+                    if (unit * 64 + 32 < n) tc_ld32(acc + unit * 64 + 32, r[1]);
                     tc_ld_wait();
                 }
-                if (i == (C::kShared ? 0 : kUnits / 2 - 1)) {
+                if (i == (C::kShared ? 0 : BN / 128 - 1)) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * (it & 1u));
                 }
-                if (there) store_columns(epi, row, tile_n * BN + unit * 32, r, sa);
+                if (row0 >= epi.M || col0 >= epi.N) continue;
+#pragma unroll
+                for (uint32_t part = 0; part < 2; ++part) {
+                    const uint32_t col = col0 + 32 * part;
+                    if (col >= epi.N) continue;
+                    float v[32];
+                    finish_columns(epi, col, min(32u, epi.N - col), r[part], s, v);
+                    const bool f32 = epi.type == B2_TYPE_F32;
+                    if (!epi.bulk || (epi.accumulate && col + 32 > epi.N)) {
+                        if (epi.bulk && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        __syncwarp();
+                        store_through(epi, row0, col, v, reinterpret_cast<float *>(slabs));
+                        continue;
+                    }
+                    if (f32 || part == 0) {   // the store that read this slab last is through with it
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlabs - 1) : "memory");
+                        __syncwarp();
+                    }
+                    const uint32_t slab = smem_u32(slabs) + turn * 4096, slab_row = slab + lane * 128;
+                    if (f32) {
+                        if (epi.accumulate && row < epi.M) add_old(epi, row, col, v);
+#pragma unroll
+                        for (uint32_t k = 0; k < 8; ++k)
+                            st_shared_16(slab_row + ((k ^ (lane & 7u)) << 4), __float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]),
+                                         __float_as_uint(v[4 * k + 2]), __float_as_uint(v[4 * k + 3]));
+                    } else {
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) w[j] = pack_operands(v[8 * k + 2 * j], v[8 * k + 2 * j + 1], epi.type == B2_TYPE_F16);
+                            st_shared_16(slab_row + (((4 * part + k) ^ (lane & 7u)) << 4), w[0], w[1], w[2], w[3]);
+                        }
+                        if (part == 0 && col + 32 < epi.N) continue;
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tma_store_2d(reinterpret_cast<uint64_t>(&map_c), slab, (int)(f32 ? col : col0), (int)row0);
+                    turn = turn + 1 == kSlabs ? 0 : turn + 1;
+                }
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncthreads();
     if (*abort_flag) {
@@ -315,6 +386,162 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
         if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::kTmemCols) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::kTmemCols) : "memory");
     }
+}
+
+// ---- few rows of A -----------------------------------------------------------------------------------------------------
+// Up to 256 rows of A against all of B, which is read once: a CTA takes 128 rows of B as the MMA's M side and the rows of A as
+// its N side, and where that leaves SMs without work, the CTAs of a cluster share K and add up their parts through distributed
+// shared memory, in the order of their ranks.
+constexpr uint32_t kFewRows = 256;
+constexpr uint32_t kFewSplit = 8;       // CTAs of a cluster at most
+constexpr uint32_t kFewMaxStages = 12;
+constexpr uint32_t kFewControl = 256;
+constexpr int kFewThreads = 256;
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+struct FewShape {
+    uint32_t K;
+    uint32_t n;            // rows of A, rounded up to a multiple of 8
+    uint32_t bands;        // of 128 rows of A
+    uint32_t split;        // CTAs of a cluster
+    uint32_t stages;       // of the pipeline
+    uint32_t tmem_cols;
+};
+
+__global__ void __launch_bounds__(kFewThreads)
+k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
+          const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ Epilogue epi, const __grid_constant__ FewShape shape) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t n = shape.n, split = shape.split, pipe = shape.stages;
+    // a stage: 128 rows of B, the rows of A, their scales
+    const uint32_t at_a = 128 * 128, at_sb = at_a + n * 128, at_sa = at_sb + kScaleBand, stage_bytes = at_sa + shape.bands * kScaleBand;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem);   // the control region comes first: results overwrite the stages
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kFewMaxStages + 1);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    static_assert((2 * kFewMaxStages + 1) * 8 + 8 <= kFewControl, "control region");
+    const uint32_t stage0 = smem_u32(smem) + 1024;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = split > 1 ? cluster_cta_rank() : 0u, tile = blockIdx.x / split;
+    const uint32_t bar0 = smem_u32(bars);
+    auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (kFewMaxStages + s); };
+    const uint32_t done_bar = bar0 + 8u * (2 * kFewMaxStages);
+    // this CTA's part of K, in stages
+    const uint32_t all = (shape.K + kStageK - 1) / kStageK;
+    const uint32_t kb0 = all * rank / split, kb1 = all * (rank + 1) / split;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < pipe; ++s) {
+            mbar_init(full_bar(s), 2);
+            mbar_init(empty_bar(s), 1);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sa) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sb) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(shape.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    stream_enter();
+
+    if (warp == 0 || warp == 2) {
+        if (lane == 0) {
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                const uint32_t i = kb - kb0, stage = i % pipe, phase = i / pipe & 1u;
+                if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) break;
+                const uint32_t dst = stage0 + stage * stage_bytes;
+                if (warp == 0) {
+                    mbar_expect_tx(full_bar(stage), 128 * 128 + kScaleBand);
+                    tma_load_2d<false>(dst, reinterpret_cast<uint64_t>(&map_b), full_bar(stage), (int)(kb * 128), (int)(tile * 128));
+                    tma_load_2d<false>(dst + at_sb, reinterpret_cast<uint64_t>(&map_sb), full_bar(stage), (int)(kb * (kScaleBand / 8)), (int)tile);
+                } else {
+                    mbar_expect_tx(full_bar(stage), n * 128 + shape.bands * kScaleBand);
+                    tma_load_2d<false>(dst + at_a, reinterpret_cast<uint64_t>(&map_a), full_bar(stage), (int)(kb * 128), 0);
+                    tma_load_2d<false>(dst + at_sa, reinterpret_cast<uint64_t>(&map_sa), full_bar(stage), (int)(kb * (kScaleBand / 8)), 0);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0), idesc = fp4_instr_desc(128, n);
+        const uint32_t sb_col = tmem + (n + 31) / 32 * 32, sa_col = sb_col + 16;
+        const uint64_t desc0 = smem_desc(stage0, 0, 1024), sdesc0 = scale_desc(stage0);
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            const uint32_t i = kb - kb0, stage = i % pipe, phase = i / pipe & 1u;
+            if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag))) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint64_t bd = desc0 + (stage * stage_bytes >> 4), ad = bd + (at_a >> 4);
+                const uint64_t sbd = sdesc0 + ((stage * stage_bytes + at_sb) >> 4), sad = sdesc0 + ((stage * stage_bytes + at_sa) >> 4);
+                const uint32_t steps = min(4u, (shape.K - kb * kStageK + 63u) / 64u);
+                for (uint32_t j = 0; j < steps; ++j) {
+                    tc_copy_scales<false>(sb_col + 4 * j, sbd + j * (kScaleTile >> 4));
+                    for (uint32_t b = 0; b < shape.bands; ++b)
+                        tc_copy_scales<false>(sa_col + 4 * (j * shape.bands + b), sad + ((b * kScaleBand + j * kScaleTile) >> 4));
+                }
+                for (uint32_t j = 0; j < steps; ++j)
+                    tc_mma_fp4<false>(tmem, bd + 2 * j, ad + 2 * j, idesc, sb_col + 4 * j, sa_col + 4 * j * shape.bands, kb != kb0 || j != 0 ? 1u : 0u);
+                tc_commit<false>(empty_bar(stage));
+                if (kb + 1 == kb1) tc_commit<false>(done_bar);
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4) {
+        const uint32_t q = warp & 3, col_n = tile * 128 + 32 * q + lane;   // a row of B: a column of C
+        if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag))) {
+            tc_fence_after();
+            const float sb = col_n < epi.N ? epi.scale_b[epi.b_rows ? col_n : 0] : 0.0f;
+            const float bias = epi.bias && col_n < epi.N ? epi.bias[col_n] : 0.0f;
+            float *sums = reinterpret_cast<float *>(smem + 1024);   // [row of A][128]; the MMAs have read all there was
+            for (uint32_t j0 = 0; j0 < epi.M; j0 += 16) {
+                uint32_t r[16];
+                tc_ld16(tmem_base + ((32u * q) << 16) + j0, r);
+                tc_ld_wait();
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    if (j0 + j >= epi.M) break;
+                    if (split > 1) sums[(j0 + j) * 128 + 32 * q + lane] = __uint_as_float(r[j]);
+                    else if (col_n < epi.N) store_value(epi, j0 + j, col_n, __uint_as_float(r[j]) * (epi.scale_a[epi.a_rows ? j0 + j : 0] * sb) + bias);
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 4096; ++i) __nanosleep(512);   // what is in flight lands
+        if (threadIdx.x == 0) atomicExch(&g_fp4_status, 1u);
+        __syncthreads();
+    }
+    if (split > 1) {
+        cluster_sync_all();
+        const uint32_t at = threadIdx.x & 127u, col_n = tile * 128 + at;
+        if (col_n < epi.N && !*abort_flag) {
+            const float sb = epi.scale_b[epi.b_rows ? col_n : 0], bias = epi.bias ? epi.bias[col_n] : 0.0f;
+            for (uint32_t j = rank * 2 + threadIdx.x / 128; j < epi.M; j += split * 2) {
+                float v = 0.0f;
+                for (uint32_t p = 0; p < split; ++p) v += ld_cluster_f32(map_to_cta(stage0 + (j * 128 + at) * 4, p));
+                store_value(epi, j, col_n, v * (epi.scale_a[epi.a_rows ? j : 0] * sb) + bias);
+            }
+        }
+        cluster_sync_all();
+    }
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(shape.tmem_cols) : "memory");
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -350,6 +577,17 @@ bool scales_map(CUtensorMap *m, const b2_nvfp4_operand &o, uint32_t box_bands) {
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// C: boxes of 32 rows x 128 bytes, as the epilogue's slabs hold them.
+bool result_map(CUtensorMap *m, const b2_matrix &c) {
+    const EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    const uint32_t size = c.type == B2_TYPE_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {c.cols, c.rows}, strides[1] = {c.ld * size};
+    const cuuint32_t box[2] = {128 / size, 32}, step[2] = {1, 1};
+    return fn(m, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, c.data, dims, strides, box, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Raises a kernel's limit of shared memory on the current device, once; `done`: the devices on which it has been.
 template <typename K>
 cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done) {
@@ -363,13 +601,14 @@ cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done) {
 }
 
 template <bool PAIR, int BN>
-cudaError_t gemm_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const Epilogue &epi, int sm_count, cudaStream_t s) {
+cudaError_t gemm_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c, const Epilogue &epi, int sm_count, cudaStream_t s) {
     using C = FCfg<PAIR, BN>;
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_smem(k_fp4_gemm<PAIR, BN>, C::kSmemBytes, done);
     if (e != cudaSuccess) return e;
-    CUtensorMap map_a, map_b, map_sa, map_sb;
-    if (!codes_map(&map_a, a, 128) || !codes_map(&map_b, b, C::kBRows) || !scales_map(&map_sa, a, 1) || !scales_map(&map_sb, b, C::kBands))
+    CUtensorMap map_a, map_b, map_sa, map_sb, map_c = {};
+    if (!codes_map(&map_a, a, 128) || !codes_map(&map_b, b, C::kBRows) || !scales_map(&map_sa, a, 1) || !scales_map(&map_sb, b, C::kBands) ||
+        (epi.bulk && !result_map(&map_c, c)))
         return cudaErrorInvalidValue;
     const uint32_t tiles_m = (a.rows + C::kTileM - 1) / C::kTileM, tiles_n = (b.rows + BN - 1) / BN;
     const uint64_t tiles = (uint64_t)tiles_m * tiles_n;
@@ -389,7 +628,51 @@ cudaError_t gemm_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, cons
     cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = s;
-    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<PAIR, BN>, map_a, map_b, map_sa, map_sb, epi, a.cols, tiles_m, (uint32_t)tiles);
+    return cudaLaunchKernelEx(&cfg, k_fp4_gemm<PAIR, BN>, map_a, map_b, map_sa, map_sb, map_c, epi, a.cols, tiles_m, (uint32_t)tiles);
+}
+
+cudaError_t few_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const Epilogue &epi, int sm_count, cudaStream_t s) {
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(k_fp4_few, (uint32_t)kSmemLimit, done);
+    if (e != cudaSuccess) return e;
+    FewShape f = {};
+    f.K = a.cols;
+    f.n = (a.rows + 7) / 8 * 8;
+    f.bands = (a.rows + 127) / 128;
+    const uint32_t tiles = (b.rows + 127) / 128, all = (a.cols + kStageK - 1) / kStageK;
+    f.split = std::max(1u, std::min({kFewSplit, all, (uint32_t)sm_count / tiles}));
+#ifdef B2_MEASURE
+    if (const char *v = getenv("B2_FP4_SPLIT")) f.split = std::min((uint32_t)atoi(v), all);
+#endif
+    const uint32_t stage_bytes = 128 * 128 + f.n * 128 + (1 + f.bands) * kScaleBand;
+    // the partial sums lie where the stages were
+    const uint32_t sums = f.split > 1 ? a.rows * 512 : 0, most = ((uint32_t)kSmemLimit - 2048) / stage_bytes;
+    f.stages = std::min({kFewMaxStages, most, (all + f.split - 1) / f.split});
+    f.tmem_cols = 32;
+    while (f.tmem_cols < (f.n + 31) / 32 * 32 + 16 + 16 * f.bands) f.tmem_cols *= 2;
+    // A CTA keeps its tensor memory while it waits for the others of its cluster, so none of them may have to wait for tensor
+    // memory in turn: every launch takes at least the share of an SM's shared memory (228 KB, 1 KB of it for the system) that it
+    // takes of the tensor memory, and more than a Newton-Schulz CTA that holds all of it leaves.
+    const uint32_t share = 228u * 1024 / 512 * f.tmem_cols - 1024;
+    const uint32_t bytes = std::max({2048 + std::max(f.stages * stage_bytes, sums), share, 40u * 1024});
+    CUtensorMap map_a, map_b, map_sa, map_sb;
+    if (!codes_map(&map_a, a, f.n) || !codes_map(&map_b, b, 128) || !scales_map(&map_sa, a, f.bands) || !scales_map(&map_sb, b, 1))
+        return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = f.split;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = f.split > 1 ? 2 : 1;
+    cfg.gridDim = dim3(tiles * f.split);
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, k_fp4_few, map_a, map_b, map_sa, map_sb, epi, f);
 }
 
 }  // namespace
@@ -409,8 +692,20 @@ cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand 
     epi.b_rows = b.scale_count != 1;
     epi.type = c.type;
     epi.accumulate = accumulate;
-    epi.vec = reinterpret_cast<uintptr_t>(c.data) % 32 == 0 && epi.pitch % 32 == 0;
-    return gemm_impl<false, 128>(a, b, epi, sm_count, s);
+    epi.bulk = reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && epi.pitch % 16 == 0;
+    epi.bias_vec = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
+#ifdef B2_MEASURE
+    if (const char *v = getenv("B2_FP4_SHAPE")) {
+        const int k = atoi(v);
+        if (k == 0 && a.rows <= kFewRows) return few_impl(a, b, epi, sm_count, s);
+        if (k == 1) return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
+        if (k == 2) return gemm_impl<true, 128>(a, b, c, epi, sm_count, s);
+        if (k == 3) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
+    }
+#endif
+    if (a.rows <= kFewRows / 2) return few_impl(a, b, epi, sm_count, s);
+    if (a.rows >= 1024) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
+    return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
 }
 
 cudaError_t fp4_gemm_status(uint32_t *status, cudaStream_t s) {

@@ -15,7 +15,7 @@ OUT_DIR = os.path.join(HERE, "_lib")
 LIB_PATH = os.path.join(OUT_DIR, "libllmini_b200.so")
 SOURCES = ["stream_kernels.cu", "ns_gemm_sm100.cu", "api.cu", "host.cu", "peer_gather.cu", "no_alloc.cu", "fp4_kernels.cu",
            "fp4_gemm_sm100.cu", "fp4_api.cu"]
-HEADERS = ["common.cuh", "internal.h", "sm100.cuh", "fp4.h", os.path.join("..", "..", "include", "llmini_b200.h"),
+HEADERS = ["common.cuh", "internal.h", "sm100.cuh", "fp4.h", "fp4_block.cuh", os.path.join("..", "..", "include", "llmini_b200.h"),
            os.path.join("..", "..", "include", "llmini_b200_fp4.h")]
 # -fmad=false: `a*b + c` is fused only where the source says fmaf, matching the reference's
 # Rust arithmetic.  B2_MEASURE=1 in the environment adds -DB2_MEASURE: the kernel variants used to

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/llmini_b200_fp4.h"
 
 namespace b2 {
@@ -25,6 +27,18 @@ inline cudaError_t overlapped_launch(void (*kernel)(P...), dim3 grid, int thread
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// Raises a kernel's limit of shared memory on the current device, once; `done`: the devices on which it has been.
+template <typename K>
+inline cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1u)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    return e;
+}
+
 // ---- fp4_kernels.cu --------------------------------------------------------------------------------------------------
 cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s);
 // Scales on top of parts of x, whose largest is the tensor's: writes `*count` (at most B2_NVFP4_MAXIMA) of them.
@@ -41,6 +55,10 @@ cudaError_t launch_fp4_cache_read(const b2_nvfp4_cache *caches, const b2_vectors
 // ---- fp4_gemm_sm100.cu -----------------------------------------------------------------------------------------------
 cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias,
                               bool accumulate, int sm_count, cudaStream_t s);
+// x quantised by rows on the way, for few values (fp4_linear_fused).
+bool fp4_linear_fused(uint32_t rows, uint32_t cols);
+cudaError_t launch_fp4_linear(const b2_matrix &x, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias, int sm_count,
+                              cudaStream_t s);
 cudaError_t fp4_gemm_status(uint32_t *status, cudaStream_t s);
 
 }  // namespace b2

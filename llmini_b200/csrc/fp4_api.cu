@@ -116,6 +116,9 @@ int b2_nvfp4_linear_forward(const b2_matrix *x, const b2_nvfp4_operand *weight, 
     if (y->rows == 0 || y->cols == 0) return B2_SUCCESS;
     int sms = 0;
     cudaError_t e = sm_count(sms);
+    // a few values are quantised by every CTA of the product for itself; more, once
+    if (e == cudaSuccess && b2::fp4_linear_fused(x->rows, x->cols))
+        return (int)b2::launch_fp4_linear(*x, *weight, *y, d_bias, sms, as_stream(stream));
     if (e == cudaSuccess) e = launch_fp4_quantize_rows(*x, *scratch, as_stream(stream));
     if (e == cudaSuccess) e = launch_fp4_matmul(*scratch, *weight, *y, d_bias, false, sms, as_stream(stream));
     return (int)e;

@@ -12,6 +12,7 @@
 
 #include "common.cuh"
 #include "fp4.h"
+#include "fp4_block.cuh"
 #include "sm100.cuh"
 
 namespace b2 {
@@ -389,65 +390,97 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
 }
 
 // ---- few rows of A -----------------------------------------------------------------------------------------------------
-// Up to 256 rows of A against all of B, which is read once: a CTA takes 128 rows of B as the MMA's M side and the rows of A as
-// its N side, and where that leaves SMs without work, the CTAs of a cluster share K and add up their parts through distributed
-// shared memory, in the order of their ranks.
-constexpr uint32_t kFewRows = 256;
+// A step of generation: up to 64 rows of A against all of B, which is read once.  A CTA takes 128 rows of B as the MMA's M side and
+// the rows of A as its N side.  Where that leaves SMs without work, the CTAs of a cluster share K: rows of A go in groups of four,
+// each CTA sends its sums of group j to the CTA of rank j % split, which adds them up in the order of the ranks.
+// TYPE >= 0: A is up to eight rows of plain values, which every CTA quantises for itself while its first tiles of B are on their
+// way, and the quantiser's launch and its way through memory are saved.
+// (The same with B decoded to FP16 for mma.sync, without tensor memory and maps, spent five instructions on a code: 31 us for
+// 1 x 1600 -> 50304, and 7.2 for 1 x 1600 -> 4800.)
+constexpr uint32_t kFewRows = 64, kFusedRows = 8;
 constexpr uint32_t kFewSplit = 8;       // CTAs of a cluster at most
 constexpr uint32_t kFewMaxStages = 12;
-constexpr uint32_t kFewControl = 256;
+constexpr uint32_t kFewControl = 1024;
 constexpr int kFewThreads = 256;
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
+__device__ __forceinline__ void st_cluster_16(uint32_t addr, const uint32_t *v) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
 
 struct FewShape {
     uint32_t K;
     uint32_t n;            // rows of A, rounded up to a multiple of 8
-    uint32_t bands;        // of 128 rows of A
     uint32_t split;        // CTAs of a cluster
     uint32_t stages;       // of the pipeline
+    uint32_t share;        // stages of K that a CTA has at most
     uint32_t tmem_cols;
+    // plain values
+    const uint8_t *x;
+    uint64_t x_pitch;      // bytes
+    uint32_t x_cols, x_vec;
 };
+// Shared memory behind the 1024 bytes of barriers and the rows' scales: the pipeline's stages; TYPE >= 0: codes and scales of the
+// rows of A for the CTA's part of K; the sums that the cluster sends.
+struct FewLayout {
+    uint32_t at_a, at_sb, at_sa, stage_bytes;   // in a stage: 128 rows of B (at 0), rows of A, scales
+    uint32_t at_x, at_xs, at_sums, bytes;
+};
+__host__ __device__ inline FewLayout few_layout(const FewShape &f, bool fused) {
+    FewLayout l;
+    l.at_a = 128 * 128;
+    l.at_sb = l.at_a + (fused ? 0u : f.n * 128);
+    l.at_sa = l.at_sb + kScaleBand;
+    l.stage_bytes = l.at_sa + (fused ? 0u : kScaleBand);
+    l.stage_bytes = (l.stage_bytes + 1023) / 1024 * 1024;
+    l.at_x = kFewControl + f.stages * l.stage_bytes;
+    l.at_xs = l.at_x + (fused ? f.share * 1024 : 0u);
+    l.at_sums = l.at_xs + (fused ? f.share * 512 + 512 : 0u);
+    l.bytes = l.at_sums + (f.split > 1 ? f.split * (((f.n + 3) / 4 + f.split - 1) / f.split) * 2048 : 0u);
+    return l;
+}
 
+template <int TYPE>
 __global__ void __launch_bounds__(kFewThreads)
 k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_sa,
           const __grid_constant__ CUtensorMap map_sb, const __grid_constant__ Epilogue epi, const __grid_constant__ FewShape shape) {
+    constexpr bool kFused = TYPE >= 0;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t n = shape.n, split = shape.split, pipe = shape.stages;
-    // a stage: 128 rows of B, the rows of A, their scales
-    const uint32_t at_a = 128 * 128, at_sb = at_a + n * 128, at_sa = at_sb + kScaleBand, stage_bytes = at_sa + shape.bands * kScaleBand;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(smem);   // the control region comes first: results overwrite the stages
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kFewMaxStages + 1);
+    const FewLayout lay = few_layout(shape, kFused);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 2 * kFewMaxStages + 2);
     volatile uint32_t *abort_flag = tmem_slot + 1;
-    static_assert((2 * kFewMaxStages + 1) * 8 + 8 <= kFewControl, "control region");
-    const uint32_t stage0 = smem_u32(smem) + 1024;
+    uint32_t *maxima = tmem_slot + 2;                              // of up to eight rows of plain values
+    float *tops = reinterpret_cast<float *>(smem + 512);           // the rows of A's scales
+    static_assert((2 * kFewMaxStages + 2) * 8 + 8 + kFusedRows * 4 <= 512 && kFewRows * 4 <= 512, "control region");
+    const uint32_t stage0 = smem_u32(smem) + kFewControl;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = split > 1 ? cluster_cta_rank() : 0u, tile = blockIdx.x / split;
     const uint32_t bar0 = smem_u32(bars);
     auto full_bar = [&](uint32_t s) { return bar0 + 8u * s; };
     auto empty_bar = [&](uint32_t s) { return bar0 + 8u * (kFewMaxStages + s); };
-    const uint32_t done_bar = bar0 + 8u * (2 * kFewMaxStages);
+    const uint32_t done_bar = bar0 + 8u * (2 * kFewMaxStages), x_bar = done_bar + 8u;
     // this CTA's part of K, in stages
     const uint32_t all = (shape.K + kStageK - 1) / kStageK;
     const uint32_t kb0 = all * rank / split, kb1 = all * (rank + 1) / split;
 
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < pipe; ++s) {
-            mbar_init(full_bar(s), 2);
+            mbar_init(full_bar(s), kFused ? 1 : 2);
             mbar_init(empty_bar(s), 1);
         }
         mbar_init(done_bar, 1);
+        mbar_init(x_bar, kFewThreads - 64);
         *abort_flag = 0;
+        for (uint32_t i = 0; i < kFusedRows; ++i) maxima[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_smem();
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        if (!kFused) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sa) : "memory");
+        }
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sa) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_sb) : "memory");
     }
     if (warp == 1) {
@@ -458,22 +491,23 @@ k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
+    if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // this CTA runs: it can be sent to
     stream_enter();
 
-    if (warp == 0 || warp == 2) {
+    if (warp == 0 || (!kFused && warp == 2)) {
         if (lane == 0) {
             for (uint32_t kb = kb0; kb < kb1; ++kb) {
                 const uint32_t i = kb - kb0, stage = i % pipe, phase = i / pipe & 1u;
                 if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) break;
-                const uint32_t dst = stage0 + stage * stage_bytes;
+                const uint32_t dst = stage0 + stage * lay.stage_bytes;
                 if (warp == 0) {
                     mbar_expect_tx(full_bar(stage), 128 * 128 + kScaleBand);
                     tma_load_2d<false>(dst, reinterpret_cast<uint64_t>(&map_b), full_bar(stage), (int)(kb * 128), (int)(tile * 128));
-                    tma_load_2d<false>(dst + at_sb, reinterpret_cast<uint64_t>(&map_sb), full_bar(stage), (int)(kb * (kScaleBand / 8)), (int)tile);
+                    tma_load_2d<false>(dst + lay.at_sb, reinterpret_cast<uint64_t>(&map_sb), full_bar(stage), (int)(kb * (kScaleBand / 8)), (int)tile);
                 } else {
-                    mbar_expect_tx(full_bar(stage), n * 128 + shape.bands * kScaleBand);
-                    tma_load_2d<false>(dst + at_a, reinterpret_cast<uint64_t>(&map_a), full_bar(stage), (int)(kb * 128), 0);
-                    tma_load_2d<false>(dst + at_sa, reinterpret_cast<uint64_t>(&map_sa), full_bar(stage), (int)(kb * (kScaleBand / 8)), 0);
+                    mbar_expect_tx(full_bar(stage), n * 128 + kScaleBand);
+                    tma_load_2d<false>(dst + lay.at_a, reinterpret_cast<uint64_t>(&map_a), full_bar(stage), (int)(kb * 128), 0);
+                    tma_load_2d<false>(dst + lay.at_sa, reinterpret_cast<uint64_t>(&map_sa), full_bar(stage), (int)(kb * (kScaleBand / 8)), 0);
                 }
             }
         }
@@ -481,45 +515,106 @@ k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0), idesc = fp4_instr_desc(128, n);
         const uint32_t sb_col = tmem + (n + 31) / 32 * 32, sa_col = sb_col + 16;
         const uint64_t desc0 = smem_desc(stage0, 0, 1024), sdesc0 = scale_desc(stage0);
-        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        bool ok = !kFused || __all_sync(0xffffffffu, mbar_wait(x_bar, 0, abort_flag));
+        for (uint32_t kb = kb0; ok && kb < kb1; ++kb) {
             const uint32_t i = kb - kb0, stage = i % pipe, phase = i / pipe & 1u;
             if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag))) break;
             tc_fence_after();
             if (elect_one()) {
-                const uint64_t bd = desc0 + (stage * stage_bytes >> 4), ad = bd + (at_a >> 4);
-                const uint64_t sbd = sdesc0 + ((stage * stage_bytes + at_sb) >> 4), sad = sdesc0 + ((stage * stage_bytes + at_sa) >> 4);
+                const uint32_t at = stage * lay.stage_bytes;
+                const uint64_t bd = desc0 + (at >> 4), sbd = sdesc0 + ((at + lay.at_sb) >> 4);
+                const uint64_t ad = kFused ? smem_desc(smem_u32(smem) + lay.at_x + i * 1024, 0, 1024) : bd + (lay.at_a >> 4);
+                const uint64_t sad = kFused ? scale_desc(smem_u32(smem) + lay.at_xs + i * 512) : sdesc0 + ((at + lay.at_sa) >> 4);
                 const uint32_t steps = min(4u, (shape.K - kb * kStageK + 63u) / 64u);
                 for (uint32_t j = 0; j < steps; ++j) {
                     tc_copy_scales<false>(sb_col + 4 * j, sbd + j * (kScaleTile >> 4));
-                    for (uint32_t b = 0; b < shape.bands; ++b)
-                        tc_copy_scales<false>(sa_col + 4 * (j * shape.bands + b), sad + ((b * kScaleBand + j * kScaleTile) >> 4));
+                    tc_copy_scales<false>(sa_col + 4 * j, sad + j * ((kFused ? 128u : kScaleTile) >> 4));
                 }
                 for (uint32_t j = 0; j < steps; ++j)
-                    tc_mma_fp4<false>(tmem, bd + 2 * j, ad + 2 * j, idesc, sb_col + 4 * j, sa_col + 4 * j * shape.bands, kb != kb0 || j != 0 ? 1u : 0u);
+                    tc_mma_fp4<false>(tmem, bd + 2 * j, ad + 2 * j, idesc, sb_col + 4 * j, sa_col + 4 * j, kb != kb0 || j != 0 ? 1u : 0u);
                 tc_commit<false>(empty_bar(stage));
                 if (kb + 1 == kb1) tc_commit<false>(done_bar);
             }
             __syncwarp();
         }
+    } else if (kFused) {
+        // Rows' maxima over all of K, then this CTA's part of K: codes as 8 rows of 128 bytes in the 128-byte swizzle for a stage, a
+        // scale tile of 128 bytes for 64 values (rows 0 .. 7; what the copy reads behind them belongs to rows that do not exist).
+        constexpr int T = kFused ? TYPE : 0;
+        const uint32_t t = threadIdx.x - 64, blocks = shape.K / 16;
+        auto load = [&](Raw<T> &r, uint32_t row, uint32_t blk) {
+            if (blk * 16 >= shape.x_cols) r.clear();
+            else r.load(shape.x + row * shape.x_pitch + (uint64_t)blk * 16 * Raw<T>::kSize, (int)min(shape.x_cols - blk * 16, 16u), shape.x_vec != 0);
+        };
+        for (uint32_t i = t; i < epi.M * blocks; i += kFewThreads - 64) {
+            Raw<T> r;
+            load(r, i / blocks, i % blocks);
+            atomicMax(maxima + i / blocks, r.amax_bits());
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(kFewThreads - 64) : "memory");
+        const uint32_t first = kb0 * (kStageK / 16), mine = min((blocks + 3) / 4 * 4, kb1 * (kStageK / 16)) - first;
+        for (uint32_t i = t; i < epi.M * mine; i += kFewThreads - 64) {
+            const uint32_t row = i / mine, blk = i % mine;
+            const float inv = top_inverse(top_scale(maxima[row]));
+            Raw<T> r;
+            load(r, row, first + blk);
+            uint2 codes;
+            const uint32_t s = encode_block([&](int k) { return r.values(k); }, r.amax_bits(), inv, codes);
+            const uint32_t in_stage = blk % (kStageK / 16);
+            *reinterpret_cast<uint2 *>(smem + lay.at_x + blk / (kStageK / 16) * 1024 + row * 128 + (((in_stage >> 1) ^ row) << 4) + (in_stage & 1u) * 8) = codes;
+            smem[lay.at_xs + blk / 4 * 128 + row * 16 + (blk & 3u)] = (uint8_t)s;
+        }
+        if (t < epi.M) tops[t] = top_scale(maxima[t]);
+        fence_async_smem();   // the tensor core reads what these threads have written
+        mbar_arrive(x_bar);
     } else if (warp >= 4) {
-        const uint32_t q = warp & 3, col_n = tile * 128 + 32 * q + lane;   // a row of B: a column of C
-        if (__all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag))) {
-            tc_fence_after();
-            const float sb = col_n < epi.N ? epi.scale_b[epi.b_rows ? col_n : 0] : 0.0f;
-            const float bias = epi.bias && col_n < epi.N ? epi.bias[col_n] : 0.0f;
-            float *sums = reinterpret_cast<float *>(smem + 1024);   // [row of A][128]; the MMAs have read all there was
-            for (uint32_t j0 = 0; j0 < epi.M; j0 += 16) {
-                uint32_t r[16];
-                tc_ld16(tmem_base + ((32u * q) << 16) + j0, r);
-                tc_ld_wait();
+        for (uint32_t j = threadIdx.x - 128; j < epi.M; j += 128) tops[j] = epi.scale_a[epi.a_rows ? j : 0];
+    }
+    bool ok = true;
+    if (warp >= 4) ok = __all_sync(0xffffffffu, mbar_wait(done_bar, 0, abort_flag));
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t groups = (epi.M + 3) / 4, held = (groups + split - 1) / split;   // groups of four rows, and those a CTA adds up
+    if (split > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp >= 4 && ok) {
+        const uint32_t q = warp & 3, at = 32 * q + lane, col_n = tile * 128 + at;   // a row of B: a column of C
+        const float sb = col_n < epi.N ? epi.scale_b[epi.b_rows ? col_n : 0] : 0.0f;
+        const float bias = epi.bias && col_n < epi.N ? epi.bias[col_n] : 0.0f;
+        const uint32_t to = smem_u32(smem) + lay.at_sums + (rank * held * 128 + at) * 16;
+        for (uint32_t j0 = 0; j0 < epi.M; j0 += 32) {
+            uint32_t r[32];
+            tc_ld32(tmem_base + ((32u * q) << 16) + j0, r);
+            tc_ld_wait();
 #pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) {
-                    if (j0 + j >= epi.M) break;
-                    if (split > 1) sums[(j0 + j) * 128 + 32 * q + lane] = __uint_as_float(r[j]);
-                    else if (col_n < epi.N) store_value(epi, j0 + j, col_n, __uint_as_float(r[j]) * (epi.scale_a[epi.a_rows ? j0 + j : 0] * sb) + bias);
+            for (uint32_t j = 0; j < 8; ++j) {
+                const uint32_t group = j0 / 4 + j;
+                if (group >= groups) break;
+                if (split > 1) {
+                    st_cluster_16(map_to_cta(to + group / split * 2048, group % split), r + 4 * j);
+                } else if (col_n < epi.N) {
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i)
+                        if (4 * group + i < epi.M) store_value(epi, 4 * group + i, col_n, __uint_as_float(r[4 * j + i]) * (tops[4 * group + i] * sb) + bias);
                 }
             }
-            tc_fence_before();
+        }
+        tc_fence_before();
+    }
+    if (split > 1) {
+        cluster_sync_all();
+        const uint32_t at = threadIdx.x & 127u, col_n = tile * 128 + at;
+        if (col_n < epi.N) {
+            const float sb = epi.scale_b[epi.b_rows ? col_n : 0], bias = epi.bias ? epi.bias[col_n] : 0.0f;
+            for (uint32_t group = rank + threadIdx.x / 128 * split; group < groups; group += 2 * split) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (uint32_t p = 0; p < split; ++p) {
+                    const float4 o = *reinterpret_cast<const float4 *>(smem + lay.at_sums + ((p * held + group / split) * 128 + at) * 16);
+                    v[0] += o.x; v[1] += o.y; v[2] += o.z; v[3] += o.w;
+                }
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (4 * group + i < epi.M) store_value(epi, 4 * group + i, col_n, v[i] * (tops[4 * group + i] * sb) + bias);
+            }
         }
     }
     __syncthreads();
@@ -527,19 +622,6 @@ k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         for (int i = 0; i < 4096; ++i) __nanosleep(512);   // what is in flight lands
         if (threadIdx.x == 0) atomicExch(&g_fp4_status, 1u);
         __syncthreads();
-    }
-    if (split > 1) {
-        cluster_sync_all();
-        const uint32_t at = threadIdx.x & 127u, col_n = tile * 128 + at;
-        if (col_n < epi.N && !*abort_flag) {
-            const float sb = epi.scale_b[epi.b_rows ? col_n : 0], bias = epi.bias ? epi.bias[col_n] : 0.0f;
-            for (uint32_t j = rank * 2 + threadIdx.x / 128; j < epi.M; j += split * 2) {
-                float v = 0.0f;
-                for (uint32_t p = 0; p < split; ++p) v += ld_cluster_f32(map_to_cta(stage0 + (j * 128 + at) * 4, p));
-                store_value(epi, j, col_n, v * (epi.scale_a[epi.a_rows ? j : 0] * sb) + bias);
-            }
-        }
-        cluster_sync_all();
     }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(shape.tmem_cols) : "memory");
 }
@@ -588,18 +670,6 @@ bool result_map(CUtensorMap *m, const b2_matrix &c) {
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Raises a kernel's limit of shared memory on the current device, once; `done`: the devices on which it has been.
-template <typename K>
-cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &done) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1u)) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
-    return e;
-}
-
 template <bool PAIR, int BN>
 cudaError_t gemm_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c, const Epilogue &epi, int sm_count, cudaStream_t s) {
     using C = FCfg<PAIR, BN>;
@@ -631,32 +701,42 @@ cudaError_t gemm_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, cons
     return cudaLaunchKernelEx(&cfg, k_fp4_gemm<PAIR, BN>, map_a, map_b, map_sa, map_sb, map_c, epi, a.cols, tiles_m, (uint32_t)tiles);
 }
 
-cudaError_t few_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const Epilogue &epi, int sm_count, cudaStream_t s) {
+// `x`: plain values in A's place (TYPE is theirs), else null
+template <int TYPE>
+cudaError_t few_impl(const b2_nvfp4_operand *a, const b2_matrix *x, const b2_nvfp4_operand &b, const Epilogue &epi, int sm_count, cudaStream_t s) {
+    constexpr bool kFused = TYPE >= 0;
     static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem(k_fp4_few, (uint32_t)kSmemLimit, done);
+    const cudaError_t e = allow_smem(k_fp4_few<TYPE>, (uint32_t)kSmemLimit, done);
     if (e != cudaSuccess) return e;
     FewShape f = {};
-    f.K = a.cols;
-    f.n = (a.rows + 7) / 8 * 8;
-    f.bands = (a.rows + 127) / 128;
-    const uint32_t tiles = (b.rows + 127) / 128, all = (a.cols + kStageK - 1) / kStageK;
+    f.K = b.cols;
+    f.n = (epi.M + 7) / 8 * 8;
+    if (kFused) {
+        f.x = static_cast<const uint8_t *>(x->data);
+        f.x_pitch = x->ld * Raw<kFused ? TYPE : 0>::kSize;
+        f.x_cols = x->cols;
+        f.x_vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && f.x_pitch % 16 == 0;
+    }
+    const uint32_t tiles = (b.rows + 127) / 128, all = (b.cols + kStageK - 1) / kStageK;
     f.split = std::max(1u, std::min({kFewSplit, all, (uint32_t)sm_count / tiles}));
 #ifdef B2_MEASURE
     if (const char *v = getenv("B2_FP4_SPLIT")) f.split = std::min((uint32_t)atoi(v), all);
 #endif
-    const uint32_t stage_bytes = 128 * 128 + f.n * 128 + (1 + f.bands) * kScaleBand;
-    // the partial sums lie where the stages were
-    const uint32_t sums = f.split > 1 ? a.rows * 512 : 0, most = ((uint32_t)kSmemLimit - 2048) / stage_bytes;
-    f.stages = std::min({kFewMaxStages, most, (all + f.split - 1) / f.split});
+    f.share = (all + f.split - 1) / f.split;
+    // where there are tiles for several CTAs an SM, a short pipeline leaves room for them
+    f.stages = std::min({kFewMaxStages, f.share, tiles * f.split > (uint32_t)sm_count ? 3u : kFewMaxStages});
+#ifdef B2_MEASURE
+    if (const char *v = getenv("B2_FP4_STAGES")) f.stages = std::min((uint32_t)atoi(v), f.share);
+#endif
+    while (f.stages > 1 && few_layout(f, kFused).bytes > (uint32_t)kSmemLimit - 1024) --f.stages;
     f.tmem_cols = 32;
-    while (f.tmem_cols < (f.n + 31) / 32 * 32 + 16 + 16 * f.bands) f.tmem_cols *= 2;
+    while (f.tmem_cols < (f.n + 31) / 32 * 32 + 32) f.tmem_cols *= 2;
     // A CTA keeps its tensor memory while it waits for the others of its cluster, so none of them may have to wait for tensor
     // memory in turn: every launch takes at least the share of an SM's shared memory (228 KB, 1 KB of it for the system) that it
     // takes of the tensor memory, and more than a Newton-Schulz CTA that holds all of it leaves.
-    const uint32_t share = 228u * 1024 / 512 * f.tmem_cols - 1024;
-    const uint32_t bytes = std::max({2048 + std::max(f.stages * stage_bytes, sums), share, 40u * 1024});
-    CUtensorMap map_a, map_b, map_sa, map_sb;
-    if (!codes_map(&map_a, a, f.n) || !codes_map(&map_b, b, 128) || !scales_map(&map_sa, a, f.bands) || !scales_map(&map_sb, b, 1))
+    const uint32_t bytes = std::max({few_layout(f, kFused).bytes + 1024, 228u * 1024 / 512 * f.tmem_cols - 1024, 40u * 1024});
+    CUtensorMap map_a = {}, map_b, map_sa = {}, map_sb;
+    if ((!kFused && (!codes_map(&map_a, *a, f.n) || !scales_map(&map_sa, *a, 1))) || !codes_map(&map_b, b, 128) || !scales_map(&map_sb, b, 1))
         return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
@@ -672,40 +752,57 @@ cudaError_t few_impl(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const
     cfg.blockDim = dim3(kFewThreads);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = s;
-    return cudaLaunchKernelEx(&cfg, k_fp4_few, map_a, map_b, map_sa, map_sb, epi, f);
+    return cudaLaunchKernelEx(&cfg, k_fp4_few<TYPE>, map_a, map_b, map_sa, map_sb, epi, f);
+}
+
+Epilogue epilogue_of(const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias, bool accumulate) {
+    Epilogue epi = {};
+    epi.c = static_cast<uint8_t *>(c.data);
+    epi.pitch = c.ld * (c.type == B2_TYPE_F32 ? 4 : 2);
+    epi.scale_b = b.scale;
+    epi.bias = bias;
+    epi.M = c.rows;
+    epi.N = c.cols;
+    epi.b_rows = b.scale_count != 1;
+    epi.type = c.type;
+    epi.accumulate = accumulate;
+    epi.bulk = reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && epi.pitch % 16 == 0;
+    epi.bias_vec = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
+    return epi;
 }
 
 }  // namespace
 
 cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias, bool accumulate,
                               int sm_count, cudaStream_t s) {
-    const uint64_t size = c.type == B2_TYPE_F32 ? 4 : 2;
-    Epilogue epi = {};
-    epi.c = static_cast<uint8_t *>(c.data);
-    epi.pitch = c.ld * size;
+    Epilogue epi = epilogue_of(b, c, bias, accumulate);
     epi.scale_a = a.scale;
-    epi.scale_b = b.scale;
-    epi.bias = bias;
-    epi.M = a.rows;
-    epi.N = b.rows;
     epi.a_rows = a.scale_count != 1;
-    epi.b_rows = b.scale_count != 1;
-    epi.type = c.type;
-    epi.accumulate = accumulate;
-    epi.bulk = reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && epi.pitch % 16 == 0;
-    epi.bias_vec = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
 #ifdef B2_MEASURE
     if (const char *v = getenv("B2_FP4_SHAPE")) {
         const int k = atoi(v);
-        if (k == 0 && a.rows <= kFewRows) return few_impl(a, b, epi, sm_count, s);
+        if (k == 0 && a.rows <= kFewRows) return few_impl<-1>(&a, nullptr, b, epi, sm_count, s);
         if (k == 1) return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
         if (k == 2) return gemm_impl<true, 128>(a, b, c, epi, sm_count, s);
         if (k == 3) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
     }
 #endif
-    if (a.rows <= kFewRows / 2) return few_impl(a, b, epi, sm_count, s);
+    // Few rows: 24 x 1600 -> 50304 takes 8.5 us, in tiles 17.6; 24 x 6400 -> 1600, eight CTAs sharing K, 5.8 and 11.0; 16 x 768 ->
+    // 2304 is even (4.1, 3.8).  From 33 rows on only a long K pays: 64 x 6400 -> 1600 7.2 and 11.1, 64 x 1600 -> 4800 7.6 and 5.5.
+    if (a.rows <= kFewRows / 2 || (a.rows <= kFewRows && a.cols >= 4096)) return few_impl<-1>(&a, nullptr, b, epi, sm_count, s);
     if (a.rows >= 1024) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
     return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
+}
+
+// Quantised on the way and as a launch of its own: 1 x 1600 -> 4800 5.3 us and 7.0, 4 x 1600 -> 4800 6.5 and 7.3, 8 x 1600 -> 4800 8.1
+// and 7.6, 1 x 6400 -> 1600 6.6 and 7.5, 2 x 6400 -> 1600 7.6 and 7.7.
+bool fp4_linear_fused(uint32_t rows, uint32_t cols) { return rows <= kFusedRows && (uint64_t)rows * cols <= 8192; }
+
+cudaError_t launch_fp4_linear(const b2_matrix &x, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias, int sm_count, cudaStream_t s) {
+    const Epilogue epi = epilogue_of(b, c, bias, false);
+    if (x.type == B2_TYPE_F32) return few_impl<B2_TYPE_F32>(nullptr, &x, b, epi, sm_count, s);
+    if (x.type == B2_TYPE_BF16) return few_impl<B2_TYPE_BF16>(nullptr, &x, b, epi, sm_count, s);
+    return few_impl<B2_TYPE_F16>(nullptr, &x, b, epi, sm_count, s);
 }
 
 cudaError_t fp4_gemm_status(uint32_t *status, cudaStream_t s) {

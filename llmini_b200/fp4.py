@@ -12,8 +12,8 @@ from dataclasses import dataclass, field
 import torch
 
 from . import _ffi
-from ._ffi import SCALES_CSF, SCALES_RAW, SCALES_SM100, check
-from .nvfp4 import Nvfp4Tensor, _stream
+from ._ffi import SCALES_RAW, SCALES_SM100, check
+from .nvfp4 import Nvfp4Tensor, _raw_stream
 
 TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 NVFP4_MAXIMA = 1024
@@ -75,29 +75,52 @@ def _refuse(what: str):
     raise ValueError(what)
 
 
-def _here(t: torch.Tensor) -> int:
+# The current device, and its current stream's handle, without the objects around them: of the 6 us that a call on small tensors
+# takes on the host, the launch itself is 2.5.
+_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _stream_of(device: int) -> int:
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _here(t: torch.Tensor, device: int) -> int:
     """The address of a tensor of the current device."""
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != device:
         _refuse(f"a tensor on {t.device}: the call works on the current CUDA device")
     return t.data_ptr()
 
 
-def _matrix(t: torch.Tensor) -> Matrix:
-    if t.dim() != 2 or t.dtype not in _TYPES:
+def _matrix(t: torch.Tensor, device: int) -> Matrix:
+    kind = _TYPES.get(t.dtype)
+    if kind is None or t.dim() != 2:
         _refuse(f"a matrix of FP32, BF16 or F16 is wanted, not {tuple(t.shape)} of {t.dtype}")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    (rows, cols), (ld, step) = t.shape, t.stride()
+    if step != 1 and cols > 1:
         _refuse("a row's values have to lie side by side")
-    ld = t.stride(0) if rows > 1 else cols
-    if ld < cols:
+    if rows <= 1:
+        ld = cols
+    elif ld < cols:
         _refuse("rows overlap")
-    return Matrix(_here(t), ld, rows, cols, _TYPES[t.dtype], 0)
+    if t.get_device() != device:
+        _refuse(f"a tensor on {t.device}: the call works on the current CUDA device")
+    return Matrix(t.data_ptr(), ld, rows, cols, kind, 0)
 
 
-def _floats(t: torch.Tensor, count: int, what: str) -> int:
+def _floats(t: torch.Tensor, count: int, what: str, device: int) -> int:
     if t.dtype != torch.float32 or t.numel() < count or not t.is_contiguous():
         _refuse(f"{what}: {count} contiguous FP32 values are wanted")
-    return _here(t)
+    return _here(t, device)
+
+
+def _operand(o: "Nvfp4Operand", device: int):
+    if o.device_index != device:
+        _refuse("an operand of another device than the current one")
+    return o.ref
+
+
+def _csf_bytes(rows: int, k: int) -> int:
+    return int(_ffi.lib().b2_csf_encoded_len(rows, k))
 
 
 def _up(n: int, step: int) -> int:
@@ -133,6 +156,7 @@ class Nvfp4Operand:
             _refuse("an operand lies on one CUDA device")
         self.device_index = b.device.index
         self.c = Operand(b.data_ptr(), self.scales.data_ptr(), self.scale.data_ptr(), row_bytes, self.rows, self.k, n, 0)
+        self.ref = C.byref(self.c)
 
     @staticmethod
     def empty(rows: int, k: int, per_row: bool = True, device="cuda") -> "Nvfp4Operand":
@@ -185,6 +209,8 @@ class Nvfp4PagedCache:
                 _refuse("a cache lies on one CUDA device")
             self.c[i] = Cache(codes.data_ptr(), scales.data_ptr(), exponents.data_ptr(), pages, page_size, heads, half * 2)
         self.device_index = sides[0][0].device.index
+        self.sizes = [(s[0].shape[2], s[0].shape[3] * 2) for s in sides]
+        self.vectors = Vectors * len(sides)
 
     @staticmethod
     def empty(pages: int, page_size: int, heads: int, dim: int, value_dim: int | None = None, device="cuda") -> "Nvfp4PagedCache":
@@ -199,102 +225,108 @@ class Nvfp4LinearModule:
     def __init__(self):
         self._lib = _lib()
 
-    @staticmethod
-    def _ref(o):
-        if o.device_index != torch.cuda.current_device():
-            _refuse("an operand of another device than the current one")
-        return C.byref(o.c)
-
     def quantize_rows(self, x: torch.Tensor, out: Nvfp4Operand) -> None:
-        check(self._lib.b2_nvfp4_quantize_rows(C.byref(_matrix(x)), self._ref(out), _stream()), "nvfp4_quantize_rows")
+        d = _device()
+        check(self._lib.b2_nvfp4_quantize_rows(C.byref(_matrix(x, d)), _operand(out, d), _stream_of(d)), "nvfp4_quantize_rows")
 
     def quantize_columns(self, x: torch.Tensor, out: Nvfp4Operand, maxima: torch.Tensor) -> None:
         """The transpose of x; `maxima`: scratch of NVFP4_MAXIMA FP32 values."""
-        check(self._lib.b2_nvfp4_quantize_columns(C.byref(_matrix(x)), self._ref(out), _floats(maxima, NVFP4_MAXIMA, "maxima"), _stream()),
+        d = _device()
+        check(self._lib.b2_nvfp4_quantize_columns(C.byref(_matrix(x, d)), _operand(out, d), _floats(maxima, NVFP4_MAXIMA, "maxima", d), _stream_of(d)),
               "nvfp4_quantize_columns")
 
     def decode(self, operand, out: torch.Tensor) -> None:
         """The values of an Nvfp4Operand, or of an Nvfp4Tensor of any scale layout, in out's type."""
-        layout, c = SCALES_SM100, None
+        d = _device()
         if isinstance(operand, Nvfp4Tensor):
             t, layout = operand, operand.scale_layout
             if (t.k // 2) % 16 and t.rows > 1:
                 _refuse("rows of k values start on 16-byte boundaries where k is a multiple of 32")
-            need = _up(t.rows, 128) * _up(t.k // 16, 4) if layout == SCALES_SM100 else t.rows * t.k // 16 if layout == SCALES_RAW else 128
+            need = _up(t.rows, 128) * _up(t.k // 16, 4) if layout == SCALES_SM100 else t.rows * t.k // 16 if layout == SCALES_RAW else _csf_bytes(t.rows, t.k)
             if t.bytes.numel() < t.rows * t.k // 2 or t.scales.numel() < need:
                 _refuse("an Nvfp4Tensor with too little memory for its rows and k")
-            c = C.byref(Operand(_here(t.bytes), _here(t.scales), _here(t.global_scale), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
-        check(self._lib.b2_nvfp4_decode(c or self._ref(operand), layout, C.byref(_matrix(out)), _stream()), "nvfp4_decode")
-
-    def _bias(self, bias, n):
-        return None if bias is None else _floats(bias, n, "bias")
+            c = C.byref(Operand(_here(t.bytes, d), _here(t.scales, d), _here(t.global_scale, d), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
+        else:
+            c, layout = _operand(operand, d), SCALES_SM100
+        check(self._lib.b2_nvfp4_decode(c, layout, C.byref(_matrix(out, d)), _stream_of(d)), "nvfp4_decode")
 
     def matmul(self, a: Nvfp4Operand, b: Nvfp4Operand, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False) -> None:
         """out [a.rows, b.rows] = a b^T (+ bias) (+ out, FP32 only)."""
-        check(self._lib.b2_nvfp4_matmul(self._ref(a), self._ref(b), C.byref(_matrix(out)), self._bias(bias, b.rows), int(accumulate), _stream()),
-              "nvfp4_matmul")
+        d = _device()
+        check(self._lib.b2_nvfp4_matmul(_operand(a, d), _operand(b, d), C.byref(_matrix(out, d)),
+                                        None if bias is None else _floats(bias, b.rows, "bias", d), int(accumulate), _stream_of(d)), "nvfp4_matmul")
 
     def linear_forward(self, x: torch.Tensor, weight: Nvfp4Operand, out: torch.Tensor, scratch: Nvfp4LinearScratch,
                        bias: torch.Tensor | None = None) -> None:
         """out [tokens, outputs] = Q(x) weight^T (+ bias)."""
+        d = _device()
         if scratch.rows is None:
             _refuse("scratch of the backward pass")
-        check(self._lib.b2_nvfp4_linear_forward(C.byref(_matrix(x)), self._ref(weight), C.byref(_matrix(out)), self._bias(bias, weight.rows),
-                                                self._ref(scratch.rows), _stream()), "nvfp4_linear_forward")
+        check(self._lib.b2_nvfp4_linear_forward(C.byref(_matrix(x, d)), _operand(weight, d), C.byref(_matrix(out, d)),
+                                                None if bias is None else _floats(bias, weight.rows, "bias", d), _operand(scratch.rows, d),
+                                                _stream_of(d)), "nvfp4_linear_forward")
 
     def linear_backward(self, grad: torch.Tensor, x: torch.Tensor | None, weight_t: Nvfp4Operand | None, grad_x: torch.Tensor | None,
                         grad_weight: torch.Tensor | None, scratch: Nvfp4LinearScratch, accumulate: bool = False) -> None:
         """grad_x [tokens, inputs] and grad_weight [outputs, inputs] (FP32) of linear_forward; either may be None.  weight_t: the
         transposed weight, quantised along the outputs (quantize_columns of the master weights)."""
+        d = _device()
         if not scratch.backward:
             _refuse("scratch of the forward pass")
+        if (grad_x is not None and weight_t is None) or (grad_weight is not None and x is None):
+            _refuse("grad_x wants weight_t, grad_weight wants x")
         g = LinearGradients()
-        g.grad = _matrix(grad)
+        g.grad = _matrix(grad, d)
         if grad_x is not None:
-            self._ref(weight_t)
-            g.weight_t, g.grad_x = weight_t.c, _matrix(grad_x)
+            _operand(weight_t, d)
+            g.weight_t, g.grad_x = weight_t.c, _matrix(grad_x, d)
         if grad_weight is not None:
-            g.x, g.grad_weight = _matrix(x), _matrix(grad_weight)
-        self._ref(scratch.grad_rows)
+            g.x, g.grad_weight = _matrix(x, d), _matrix(grad_weight, d)
+        _operand(scratch.grad_rows, d)
         g.grad_rows, g.grad_columns, g.x_columns = scratch.grad_rows.c, scratch.grad_columns.c, scratch.x_columns.c
         g.d_maxima, g.accumulate = scratch.maxima.data_ptr(), int(accumulate)
-        check(self._lib.b2_nvfp4_linear_backward(C.byref(g), _stream()), "nvfp4_linear_backward")
+        check(self._lib.b2_nvfp4_linear_backward(C.byref(g), _stream_of(d)), "nvfp4_linear_backward")
 
     def status(self) -> int:
         """0, or ERROR_LAUNCH_TIMEOUT if a bounded device wait of a product ran out since the last call (synchronises)."""
-        return int(self._lib.b2_nvfp4_status(_stream()))
+        return int(self._lib.b2_nvfp4_status(_stream_of(_device())))
 
-    def _sides(self, cache: Nvfp4PagedCache, tensors, dims: int):
-        tensors = [t for t in tensors if t is not None]
-        if len(tensors) != len(cache.c):
-            _refuse("one tensor for each side of the cache")
-        if cache.device_index != torch.cuda.current_device():
+    @staticmethod
+    def _sides(cache: Nvfp4PagedCache, tensors, dims: int, d: int):
+        if cache.device_index != d:
             _refuse("a cache of another device than the current one")
-        v = (Vectors * len(tensors))()
-        for i, t in enumerate(tensors):
-            c = cache.c[i]
-            if t.dim() != dims or t.dtype not in _TYPES or t.dtype != tensors[0].dtype or t.shape[:-2] != tensors[0].shape[:-2]:
-                _refuse("keys and values: tensors of one type and length")
-            if t.shape[-2:] != (c.heads, c.dim) or t.stride(-1) != 1 or min(t.stride()) < 0:
+        if (tensors[1] is None) != (len(cache.c) == 1):
+            _refuse("one tensor for each side of the cache")
+        v, first, n = cache.vectors(), tensors[0], len(cache.c)
+        kind = _TYPES.get(first.dtype)
+        if kind is None or first.dim() != dims:
+            _refuse(f"vectors of FP32, BF16 or F16 are wanted, not {tuple(first.shape)} of {first.dtype}")
+        for i in range(n):
+            t, shape, stride = tensors[i], tensors[i].shape, tensors[i].stride()
+            if shape[-2:] != cache.sizes[i] or stride[-1] != 1:
                 _refuse("vectors of the cache's heads and size, their values side by side")
-            v[i] = Vectors(_here(t), t.stride(0) if dims == 4 else 0, t.stride(-3), t.stride(-2), _TYPES[t.dtype], 0)
-        return v, tensors[0]
+            if i and (t.dtype != first.dtype or shape[:-2] != first.shape[:-2]):
+                _refuse("keys and values: tensors of one type and length")
+            v[i] = Vectors(_here(t, d), stride[0] if dims == 4 else 0, stride[-3], stride[-2], kind, 0)
+        return v, n, first.shape
 
     def cache_write(self, cache: Nvfp4PagedCache, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor | None = None) -> None:
         """key, value [tokens, heads, dim] into slots int64 [tokens] (page * page_size + place; others leave a token out)."""
-        v, first = self._sides(cache, (key, value), 3)
-        if slots.dtype != torch.int64 or slots.shape != first.shape[:1] or not slots.is_contiguous():
+        d = _device()
+        v, n, shape = self._sides(cache, (key, value), 3, d)
+        if slots.dtype != torch.int64 or slots.shape != shape[:1] or not slots.is_contiguous():
             _refuse("slots: int64 [tokens]")
-        check(self._lib.b2_nvfp4_cache_write(cache.c, v, len(v), _here(slots), first.shape[0], _stream()), "nvfp4_cache_write")
+        check(self._lib.b2_nvfp4_cache_write(cache.c, v, n, _here(slots, d), shape[0], _stream_of(d)), "nvfp4_cache_write")
 
     def cache_read(self, cache: Nvfp4PagedCache, table: torch.Tensor, lengths: torch.Tensor, key: torch.Tensor,
                    value: torch.Tensor | None = None) -> None:
         """The first lengths[b] tokens of every sequence b, whose pages table [sequences, pages of a sequence] lists, into key,
         value [sequences, tokens, heads, dim]; what lies behind them is left as it is.  table, lengths: int32."""
-        v, first = self._sides(cache, (key, value), 4)
-        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] != first.shape[0]:
+        d = _device()
+        v, n, shape = self._sides(cache, (key, value), 4, d)
+        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] != shape[0]:
             _refuse("table: int32 [sequences, pages of a sequence]")
-        if lengths.dtype != torch.int32 or lengths.shape != first.shape[:1] or not lengths.is_contiguous():
+        if lengths.dtype != torch.int32 or lengths.shape != shape[:1] or not lengths.is_contiguous():
             _refuse("lengths: int32 [sequences]")
-        check(self._lib.b2_nvfp4_cache_read(cache.c, v, len(v), _here(table), table.shape[1], _here(lengths), first.shape[0], first.shape[1],
-                                            _stream()), "nvfp4_cache_read")
+        check(self._lib.b2_nvfp4_cache_read(cache.c, v, n, _here(table, d), table.shape[1], _here(lengths, d), shape[0], shape[1],
+                                            _stream_of(d)), "nvfp4_cache_read")

@@ -71,11 +71,11 @@ struct Epilogue {
     uint32_t type;             // of c
     uint32_t accumulate;
     uint32_t bulk;             // rows of c start on 16-byte boundaries: c has a tensor map
-    uint32_t bias_vec;         // the bias on a 16-byte one
 };
 
-// Sums of 32 columns from `col` on, scaled (s: the scale of A's row, and B's where it has one for all) and biased.  `n` are there.
-__device__ __forceinline__ void finish_columns(const Epilogue &e, uint32_t col, uint32_t n, const uint32_t *acc, float s, float (&v)[32]) {
+// Sums of 32 columns from `col` on, scaled (s: the scale of A's row, and B's where it has one for all) and biased (`bias`: theirs, in
+// shared memory, or null).  `n` of them are there.
+__device__ __forceinline__ void finish_columns(const Epilogue &e, uint32_t col, uint32_t n, const uint32_t *acc, float s, const float *bias, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]) * s;
     if (e.b_rows) {
@@ -83,17 +83,11 @@ __device__ __forceinline__ void finish_columns(const Epilogue &e, uint32_t col, 
         for (int i = 0; i < 32; ++i)
             if ((uint32_t)i < n) v[i] *= e.scale_b[col + i];
     }
-    if (e.bias) {
-        if (n == 32 && e.bias_vec) {
+    if (bias) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 o = reinterpret_cast<const float4 *>(e.bias + col)[i];
-                v[4 * i] += o.x; v[4 * i + 1] += o.y; v[4 * i + 2] += o.z; v[4 * i + 3] += o.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-                if ((uint32_t)i < n) v[i] += e.bias[col + i];
+        for (int i = 0; i < 8; ++i) {
+            const float4 o = reinterpret_cast<const float4 *>(bias)[i];
+            v[4 * i] += o.x; v[4 * i + 1] += o.y; v[4 * i + 2] += o.z; v[4 * i + 3] += o.w;
         }
     }
 }
@@ -158,7 +152,8 @@ struct FCfg {
     static constexpr int kProducerA = 0, kMmaWarp = 1, kEpiWarp0 = 2, kEpiWarps = 8, kProducerB = 10, kProducerS = 11;
     static constexpr int kThreads = 12 * 32;
     static constexpr uint32_t kControl = 1024;
-    static constexpr uint32_t kBesides = kControl + kEpiWarps * kSlabBytes + 1024;   // (the slabs start on a 1024-byte boundary)
+    static constexpr uint32_t kStrip = 64 * 4;   // bytes: the bias of an epilogue warp's columns
+    static constexpr uint32_t kBesides = kControl + kEpiWarps * (kSlabBytes + kStrip) + 1024;   // (the slabs start on a 1024-byte boundary)
     static constexpr uint32_t kMaxStages = ((uint32_t)kSmemLimit - kBesides) / kStageBytes;
     static constexpr uint32_t kStages = kMaxStages < 6 ? kMaxStages : 6;
     static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kBesides;
@@ -305,6 +300,7 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
         const uint32_t q = warp & 3, half = (warp - C::kEpiWarp0) >> 2;
         const uint32_t tempty_leader = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
         uint8_t *slabs = smem + C::kStages * C::kStageBytes + C::kControl + (warp - C::kEpiWarp0) * kSlabBytes;
+        float *strip = reinterpret_cast<float *>(smem + C::kStages * C::kStageBytes + C::kControl + C::kEpiWarps * kSlabBytes + (warp - C::kEpiWarp0) * C::kStrip);
         uint32_t turn = 0;
         const float sb = epi.b_rows ? 1.0f : *epi.scale_b;
         uint32_t it = 0;
@@ -313,13 +309,22 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
             const uint32_t row0 = tile_m * C::kTileM + rank * 128 + 32 * q, row = row0 + lane;
             const float s = row < epi.M ? epi.scale_a[epi.a_rows ? row : 0] * sb : 0.0f;
             const uint32_t n = mma_n(tile_n);
+            // where the accumulators share columns, these first: the last ones of the first, the first ones of the second
+            auto unit_of = [&](uint32_t i) { return C::kShared && (it & 1u) == 0 ? BN / 64 - 1 - (2 * i + half) : 2 * i + half; };
+            float bias[BN / 128][2];   // read before the tile is there
+#pragma unroll
+            for (uint32_t i = 0; i < BN / 128; ++i)
+#pragma unroll
+                for (uint32_t k = 0; k < 2; ++k) {
+                    const uint32_t col = tile_n * BN + unit_of(i) * 64 + 32 * k + lane;
+                    bias[i][k] = epi.bias && col < epi.N ? epi.bias[col] : 0.0f;
+                }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull_bar(it & 1u), (it >> 1) & 1u, abort_flag))) break;
             tc_fence_after();
             const uint32_t acc = tmem_base + (it & 1u) * C::kAcc1 + ((32u * q) << 16);
 #pragma unroll 1
             for (uint32_t i = 0; i < BN / 128; ++i) {
-                // where the accumulators share columns, these first: the last ones of the first, the first ones of the second
-                const uint32_t p = 2 * i + half, unit = C::kShared && (it & 1u) == 0 ? BN / 64 - 1 - p : p;
+                const uint32_t unit = unit_of(i);
                 const uint32_t col0 = tile_n * BN + unit * 64;
                 uint32_t r[2][32];
                 if (unit * 64 < n) {
@@ -333,12 +338,17 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                     if (lane == 0) mbar_arrive_cluster(tempty_leader + 8u * (it & 1u));
                 }
                 if (row0 >= epi.M || col0 >= epi.N) continue;
+                if (epi.bias) {
+                    strip[lane] = i == 0 ? bias[0][0] : bias[BN / 128 - 1][0];
+                    strip[lane + 32] = i == 0 ? bias[0][1] : bias[BN / 128 - 1][1];
+                    __syncwarp();
+                }
 #pragma unroll
                 for (uint32_t part = 0; part < 2; ++part) {
                     const uint32_t col = col0 + 32 * part;
                     if (col >= epi.N) continue;
                     float v[32];
-                    finish_columns(epi, col, min(32u, epi.N - col), r[part], s, v);
+                    finish_columns(epi, col, min(32u, epi.N - col), r[part], s, epi.bias ? strip + 32 * part : nullptr, v);
                     const bool f32 = epi.type == B2_TYPE_F32;
                     if (!epi.bulk || (epi.accumulate && col + 32 > epi.N)) {
                         if (epi.bulk && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -767,7 +777,6 @@ Epilogue epilogue_of(const b2_nvfp4_operand &b, const b2_matrix &c, const float 
     epi.type = c.type;
     epi.accumulate = accumulate;
     epi.bulk = reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && epi.pitch % 16 == 0;
-    epi.bias_vec = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
     return epi;
 }
 

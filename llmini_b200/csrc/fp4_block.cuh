@@ -5,11 +5,16 @@
 //   Block scale: t = RN(b / 6) for b = amax of the block / g, s = e4m3(t).  A border of the E4M3 grid has 5 bits; if b / 6 is no
 //   border, b differs from 6 borders' product by at least an ulp of b, more than half an ulp of the border: RN(b / 6) is on the
 //   right side of it, and it is the border exactly where b / 6 is.
-//   Code: q = x / g / s.  A border of the E2M1 grid times s has at most 7 bits, so the same holds for RN(q).  The quotient by
-//   s is taken with the reciprocal r = RN(1 / s) and one correction by its remainder (Markstein, IBM J. Res. Dev. 34, 1990):
-//   q0 = RN(x r), q = RN(q0 + r (x - q0 s)); the remainder is exact, so q is the quotient with a relative error of 2^-46 before
-//   its rounding.  At a border q is the border.  Off it the quotient is off by 2^-23 / 1.875 at least (s has 4 bits, so the
-//   quantity whose ulp counts has a significand of at most 1.875), 6% more than the half ulp of the border (2^-24).
+//   Code: q = x / (s g), s g exact.  A border of the E2M1 grid times s has at most 7 bits.
+//     FP32 values.  The quotient is taken with the reciprocal r = RN(1 / (s g)) and one correction by its remainder (Markstein, IBM J.
+//     Res. Dev. 34, 1990): q0 = RN(x r), q = RN(q0 + r (x - q0 s g)).  The remainder is exact (its last bit is worth 2^-35 g or
+//     more, never below 2^-145), so q is the quotient with a relative error of 2^-46 before its rounding.  At a border q is the
+//     border.  Off it the quotient is off by 2^-23 / 1.875 at least (s has 4 bits, so the quantity whose ulp counts has a
+//     significand of at most 1.875), 6% more than the half ulp of the border (2^-24).
+//     16-bit values have 11 bits at most: a quotient that is no border is 2^-11 of it away from it, 2^-13 or more.  So q is rounded
+//     to multiples of 2^-14 (by adding 1.5 2^9, one instruction with the product, and taking it away again): an error of 2^-20 in the
+//     quotient vanishes at a border and moves nothing across one, and an approximate reciprocal will do.
+// A conversion packs two codes; sign, zero and saturation are its.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -54,6 +59,11 @@ __device__ __forceinline__ float2 halves(Pair p) {
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     Pair r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
 __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
@@ -116,44 +126,67 @@ struct Raw {
     }
 };
 
-// Code bytes and scale of a block; inv = 1 / g, 0 for a vector that is not finite.
-template <typename V>
-__device__ __forceinline__ uint32_t encode_block(V values, uint32_t amax_bits, float inv, uint2 &codes) {
+// Eight values to eight codes, the first in the low half of the first byte.
+__device__ __forceinline__ uint32_t pack_codes(Pair a, Pair b, Pair c, Pair d) {
+    const float2 p = halves(a), q = halves(b), r = halves(c), t = halves(d);
+    uint32_t v;
+    asm("{ .reg .b8 a, b, c, d; cvt.rn.satfinite.e2m1x2.f32 a, %2, %1; cvt.rn.satfinite.e2m1x2.f32 b, %4, %3; "
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5; cvt.rn.satfinite.e2m1x2.f32 d, %8, %7; mov.b32 %0, {a, b, c, d}; }"
+        : "=r"(v)
+        : "f"(p.x), "f"(p.y), "f"(q.x), "f"(q.y), "f"(r.x), "f"(r.y), "f"(t.x), "f"(t.y));
+    return v;
+}
+
+// Code bytes and scale of a block; g: the scale on top, inv: 1 / g, 0 for a vector that is not finite.
+template <int TYPE>
+__device__ __forceinline__ uint32_t encode_block(const Raw<TYPE> &block, uint32_t amax_bits, float g, float inv, uint2 &codes) {
     codes = make_uint2(0u, 0u);
     if (inv == 0.0f) return 0u;
-    const uint32_t s = cvt_e4m3x2(0.0f, div_uniform(__uint_as_float(amax_bits) * inv, 6.0f, 1.0f / 6.0f)) & 0xffu;
-    const float sf = e4m3_value((uint16_t)s);
-    const float r = s == 0u ? 0.0f : __frcp_rn(sf);
-    const Pair inv2 = pair(inv, inv), r2 = pair(r, r), ns2 = pair(-sf, -sf);
-    uint32_t b[8];
+    const float b = __uint_as_float(amax_bits) * inv, t = b * (1.0f / 6.0f);
+    const uint32_t s = cvt_e4m3x2(0.0f, fmaf(fmaf(-t, 6.0f, b), 1.0f / 6.0f, t)) & 0xffu;
+    if (s == 0u) return 0u;
+    const float step = e4m3_value((uint16_t)s) * g;
+    Pair q[8];
+    if (TYPE == B2_TYPE_F32) {
+        const float r = __frcp_rn(step);
+        const Pair r2 = pair(r, r), n2 = pair(-step, -step);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const Pair x = mul2(values(i), inv2);
-        const Pair q = mul2(x, r2);
-        const float2 v = halves(fma2(fma2(q, ns2, x), r2, q));
-        b[i] = cvt_e2m1x2(v.y, v.x);
+        for (int i = 0; i < 8; ++i) {
+            const Pair x = block.values(i), q0 = mul2(x, r2);
+            q[i] = fma2(fma2(q0, n2, x), r2, q0);
+        }
+    } else {
+        const float r = rcp_approx_ftz(step);
+        const Pair r2 = pair(r, r), c = pair(768.0f, 768.0f), nc = pair(-768.0f, -768.0f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = add2(fma2(block.values(i), r2, c), nc);
     }
-    codes.x = b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24);
-    codes.y = b[4] | (b[5] << 8) | (b[6] << 16) | (b[7] << 24);
+    codes.x = pack_codes(q[0], q[1], q[2], q[3]);
+    codes.y = pack_codes(q[4], q[5], q[6], q[7]);
     return s;
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ __half2 e2m1_values(uint32_t byte) {
-    uint32_t r;
-    asm("{ .reg .b8 t; cvt.u8.u16 t, %1; cvt.rn.f16x2.e2m1x2 %0, t; }" : "=r"(r) : "h"((uint16_t)byte));
-    return *reinterpret_cast<__half2 *>(&r);
-}
 // Values of a block: code * s is exact in FP16 (6 bits, 2^-10 .. 2688), the product with g is rounded in FP32.
 __device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, float (&v)[16]) {
     uint32_t sh;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(sh) : "h"((uint16_t)(s | (s << 8))));
     const __half2 s2 = *reinterpret_cast<const __half2 *>(&sh);
+    const Pair g2 = pair(g, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float2 f = __half22float2(__hmul2(e2m1_values((i < 4 ? codes.x : codes.y) >> (8 * (i & 3)) & 0xffu), s2));
-        v[2 * i] = f.x * g;
-        v[2 * i + 1] = f.y * g;
+    for (int k = 0; k < 2; ++k) {
+        uint32_t h[4];
+        asm("{ .reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b; "
+            "cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d; }"
+            : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+            : "r"(k ? codes.y : codes.x));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(__hmul2(*reinterpret_cast<const __half2 *>(&h[i]), s2));
+            const float2 o = halves(mul2(pair(f.x, f.y), g2));
+            v[8 * k + 2 * i] = o.x;
+            v[8 * k + 2 * i + 1] = o.y;
+        }
     }
 }
 // `n` values (at most 16) to element `p` on; `vec`: p is on a 16-byte boundary

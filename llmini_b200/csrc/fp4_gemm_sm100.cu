@@ -565,11 +565,11 @@ k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t first = kb0 * (kStageK / 16), mine = min((blocks + 3) / 4 * 4, kb1 * (kStageK / 16)) - first;
         for (uint32_t i = t; i < epi.M * mine; i += kFewThreads - 64) {
             const uint32_t row = i / mine, blk = i % mine;
-            const float inv = top_inverse(top_scale(maxima[row]));
+            const float g = top_scale(maxima[row]), inv = top_inverse(g);
             Raw<T> r;
             load(r, row, first + blk);
             uint2 codes;
-            const uint32_t s = encode_block([&](int k) { return r.values(k); }, r.amax_bits(), inv, codes);
+            const uint32_t s = encode_block(r, r.amax_bits(), g, inv, codes);
             const uint32_t in_stage = blk % (kStageK / 16);
             *reinterpret_cast<uint2 *>(smem + lay.at_x + blk / (kStageK / 16) * 1024 + row * 128 + (((in_stage >> 1) ^ row) << 4) + (in_stage & 1u) * 8) = codes;
             smem[lay.at_xs + blk / 4 * 128 + row * 16 + (blk & 3u)] = (uint8_t)s;

@@ -56,7 +56,7 @@ k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t
     if (there && in_row == 0) scale[row] = g;
     auto store = [&](const Raw<TYPE> &r, uint32_t blk) {
         uint2 codes;
-        uint32_t s = encode_block([&](int i) { return r.values(i); }, r.amax_bits(), inv, codes);
+        uint32_t s = encode_block(r, r.amax_bits(), g, inv, codes);
         if (there && blk < blocks) *reinterpret_cast<uint2 *>(bytes + (uint64_t)row * row_bytes + (uint64_t)blk * 8) = codes;
         s |= __shfl_down_sync(0xffffffffu, s, 1) << 8;   // four blocks' scales, one word of a 512-byte tile
         s |= __shfl_down_sync(0xffffffffu, s, 2) << 16;
@@ -78,7 +78,7 @@ k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t
 // ---- by columns -------------------------------------------------------------------------------------------------------------
 // Scales on top of parts of the tensor.  Rows without gaps are one row.
 template <int TYPE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 6)
 k_fp4_maxima(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint64_t cols, bool vec, float *maxima) {
     stream_enter();
     __shared__ uint32_t part[8];
@@ -176,7 +176,7 @@ k_fp4_quantize_columns(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint3
                 else r.w[i] = __byte_perm(w[(2 * i) % 16][j >> 1], w[(2 * i + 1) % 16][j >> 1], j & 1 ? 0x7632 : 0x5410);
             }
             uint2 codes;
-            const uint32_t s = encode_block([&](int i) { return r.values(i); }, r.amax_bits(), inv, codes);
+            const uint32_t s = encode_block(r, r.amax_bits(), g, inv, codes);
             const uint32_t c = lane * 4 + j;
             codes_tile[c * 8 + (warp ^ (lane & 7u))] = codes;
             scales_tile[(warp >> 2) * 512 + (c & 31u) * 16 + (c >> 5) * 4 + (warp & 3u)] = (uint8_t)s;
@@ -218,32 +218,49 @@ k_fp4_decode(const uint8_t *bytes, uint64_t row_bytes, const uint8_t *scales, ui
 }
 
 // ---- the paged cache --------------------------------------------------------------------------------------------------------
-// A vector's blocks lie in `group` neighbouring lanes (a power of two, at least dim / 16 of them up to a warp; vectors of more
-// than 512 values take two blocks a lane), which share its maximum.  blockIdx.y is the tensor: keys, values.
-struct CachePair {
-    b2_nvfp4_cache cache[2];
-    b2_vectors vectors[2];
-    bool vec[2];
+// Quotients by a divisor of the launch, for dividends below 2^31: with 2^(l-1) < d <= 2^l and m = floor(2^(31+l) / d) + 1 the
+// product n m exceeds n 2^(31+l) / d by n at most, less than what is missing to the next multiple of 2^(31+l).
+struct Divisor {
+    uint32_t d, m, shift;
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return d == 1u ? n : __umulhi(n, m) >> shift; }
 };
-template <int TYPE>
+Divisor divisor(uint32_t d) {
+    uint32_t l = 0;
+    while ((1ull << l) < d) ++l;
+    return {d, d == 1 ? 0u : (uint32_t)((1ull << (31 + l)) / d + 1), d == 1 ? 0u : l - 1};
+}
+// blockIdx.y is the tensor: keys, values.
+struct CacheSide {
+    b2_nvfp4_cache cache;
+    b2_vectors vectors;
+    Divisor heads, blocks;
+    uint32_t group;   // lanes of a vector when it is written
+    bool vec;
+};
+struct CachePair {
+    CacheSide side[2];
+    Divisor page_size[2];
+};
+// A vector's blocks lie in `group` neighbouring lanes (a power of two, at least dim / 16 of them up to a warp; TWO: vectors of more
+// than 512 values take two blocks a lane), which share its maximum.
+template <int TYPE, bool TWO>
 __global__ void __launch_bounds__(256)
-k_fp4_cache_write(const __grid_constant__ CachePair p, const int64_t *slots, uint32_t token_count, uint32_t group) {
+k_fp4_cache_write(const __grid_constant__ CachePair p, const int64_t *slots, uint32_t token_count) {
     stream_enter();
-    const b2_nvfp4_cache &c = p.cache[blockIdx.y];
-    const b2_vectors &in = p.vectors[blockIdx.y];
-    const uint64_t vector = (uint64_t)blockIdx.x * (256u / group) + threadIdx.x / group;
-    const uint32_t lane = threadIdx.x % group, blocks = c.dim / 16;
-    const uint32_t token = (uint32_t)min(vector / c.heads, (uint64_t)0xffffffffu), head = (uint32_t)(vector % c.heads);
+    const CacheSide &side = p.side[blockIdx.y];
+    const b2_nvfp4_cache &c = side.cache;
+    const uint32_t group = side.group, vector = (blockIdx.x * 256u + threadIdx.x) / group, lane = threadIdx.x & (group - 1);
+    const uint32_t blocks = side.blocks.d, token = side.heads.of(vector), head = vector - token * c.heads;
     int64_t slot = -1;
     if (token < token_count) slot = slots[token];
     const bool there = slot >= 0 && slot < (int64_t)c.pages * c.page_size;
-    const uint8_t *src = static_cast<const uint8_t *>(in.data) + (token * in.token_stride + head * in.head_stride) * Raw<TYPE>::kSize;
-    Raw<TYPE> r[2];
+    const uint8_t *src = static_cast<const uint8_t *>(side.vectors.data) + (token * side.vectors.token_stride + head * side.vectors.head_stride) * Raw<TYPE>::kSize;
+    Raw<TYPE> r[TWO ? 2 : 1];
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < (TWO ? 2 : 1); ++i) {
         const uint32_t blk = lane + i * group;
-        if (there && blk < blocks) r[i].load(src + (uint64_t)blk * 16 * Raw<TYPE>::kSize, 16, p.vec[blockIdx.y]);
+        if (there && blk < blocks) r[i].load(src + blk * 16 * Raw<TYPE>::kSize, 16, side.vec);
         else r[i].clear();
         m = max_bits(m, r[i].amax_bits());
     }
@@ -253,47 +270,49 @@ k_fp4_cache_write(const __grid_constant__ CachePair p, const int64_t *slots, uin
     const uint64_t at = (uint64_t)slot * c.heads + head;
     if (lane == 0) c.exponents[at] = (uint8_t)(__float_as_uint(g) >> 23);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < (TWO ? 2 : 1); ++i) {
         const uint32_t blk = lane + i * group;
         if (blk >= blocks) break;
         uint2 codes;
-        const Raw<TYPE> &block = r[i];
-        const uint32_t s = encode_block([&](int k) { return block.values(k); }, block.amax_bits(), inv, codes);
+        const uint32_t s = encode_block(r[i], r[i].amax_bits(), g, inv, codes);
         *reinterpret_cast<uint2 *>(c.bytes + (at * blocks + blk) * 8) = codes;
         c.scales[at * blocks + blk] = (uint8_t)s;
     }
 }
 
-// One CTA takes blocks of one sequence's tokens; a thread reads a block.
+// One CTA takes some tokens of a sequence; a thread reads a block at a time.
 template <int TYPE>
 __global__ void __launch_bounds__(256)
 k_fp4_cache_read(const __grid_constant__ CachePair p, const int32_t *table, uint32_t table_width, const int32_t *lengths,
                  uint32_t max_tokens, uint32_t tokens_per_cta) {
     stream_enter();
-    const b2_nvfp4_cache &c = p.cache[blockIdx.y];
-    const b2_vectors &out = p.vectors[blockIdx.y];
-    const uint32_t sequence = blockIdx.z, blocks = c.dim / 16, per_token = c.heads * blocks;
+    const CacheSide &side = p.side[blockIdx.y];
+    const b2_nvfp4_cache &c = side.cache;
+    const uint32_t sequence = blockIdx.z, blocks = side.blocks.d, per_token = c.heads * blocks;
     const uint64_t most = min((uint64_t)max_tokens, (uint64_t)table_width * c.page_size);
     const int32_t length = lengths[sequence];
     const uint32_t tokens = length <= 0 ? 0u : (uint32_t)min((uint64_t)length, most);
     const uint32_t t0 = blockIdx.x * tokens_per_cta;
     if (t0 >= tokens) return;
     const uint32_t work = min(tokens_per_cta, tokens - t0) * per_token;
+    const int32_t *pages = table + (uint64_t)sequence * table_width;
+    uint8_t *out = static_cast<uint8_t *>(side.vectors.data) + sequence * side.vectors.sequence_stride * Raw<TYPE>::kSize;
+#pragma unroll 2
     for (uint32_t i = threadIdx.x; i < work; i += 256) {
-        const uint32_t t = t0 + i / per_token, rest = i % per_token, head = rest / blocks, blk = rest % blocks;
-        const int32_t page = table[(uint64_t)sequence * table_width + t / c.page_size];
+        const uint32_t vector = side.blocks.of(i), blk = i - vector * blocks, token = side.heads.of(vector), head = vector - token * c.heads;
+        const uint32_t t = t0 + token, in = p.page_size[blockIdx.y].of(t);
+        const int32_t page = pages[in];
         uint2 codes = make_uint2(0u, 0u);
         uint32_t s = 0, e = 255;
         if (page >= 0 && (uint32_t)page < c.pages) {
-            const uint64_t at = ((uint64_t)page * c.page_size + t % c.page_size) * c.heads + head;
+            const uint64_t at = ((uint64_t)page * c.page_size + (t - in * c.page_size)) * c.heads + head;
             codes = *reinterpret_cast<const uint2 *>(c.bytes + (at * blocks + blk) * 8);
             s = c.scales[at * blocks + blk];
             e = c.exponents[at];
         }
         float v[16];
         decode_block(codes, s, e == 255u ? __uint_as_float(0x7fffffffu) : e == 0u ? 0x1p-127f : __uint_as_float(e << 23), v);
-        store_block<TYPE>(static_cast<uint8_t *>(out.data) + (sequence * out.sequence_stride + t * out.token_stride + head * out.head_stride + blk * 16ull) * Raw<TYPE>::kSize,
-                          v, 16, p.vec[blockIdx.y]);
+        store_block<TYPE>(out + (t * side.vectors.token_stride + head * side.vectors.head_stride + blk * 16) * Raw<TYPE>::kSize, v, 16, side.vec);
     }
 }
 
@@ -354,31 +373,37 @@ cudaError_t decode_impl(const b2_nvfp4_operand &in, uint32_t layout, const b2_ma
 CachePair cache_pair(const b2_nvfp4_cache *caches, const b2_vectors *vectors, uint32_t count) {
     CachePair p = {};
     for (uint32_t i = 0; i < count; ++i) {
-        p.cache[i] = caches[i];
-        p.vectors[i] = vectors[i];
+        CacheSide &side = p.side[i];
+        side.cache = caches[i];
+        side.vectors = vectors[i];
+        side.heads = divisor(caches[i].heads);
+        side.blocks = divisor(caches[i].dim / 16);
+        p.page_size[i] = divisor(caches[i].page_size);
+        for (side.group = 1; side.group < side.blocks.d && side.group < 32;) side.group *= 2;
         const uint64_t size = type_size(vectors[i].type);
         const uint64_t strides = (vectors[i].sequence_stride | vectors[i].token_stride | vectors[i].head_stride) * size;
-        p.vec[i] = aligned(vectors[i].data, strides, 16);
+        side.vec = aligned(vectors[i].data, strides, 16);
     }
     return p;
 }
 template <int TYPE>
 cudaError_t write_impl(const CachePair &p, uint32_t count, const int64_t *slots, uint32_t token_count, cudaStream_t s) {
-    uint32_t blocks = 0, heads = 0, group = 1;
+    uint64_t threads = 0;
+    bool two = false;
     for (uint32_t i = 0; i < count; ++i) {
-        blocks = std::max(blocks, p.cache[i].dim / 16);
-        heads = std::max(heads, p.cache[i].heads);
+        threads = std::max(threads, (uint64_t)token_count * p.side[i].cache.heads * p.side[i].group);
+        two = two || p.side[i].blocks.d > 32;
     }
-    while (group < blocks && group < 32) group *= 2;
-    const uint64_t grid = ((uint64_t)token_count * heads + 256 / group - 1) / (256 / group);
-    if (grid > 0x7fffffffu) return cudaErrorInvalidValue;
-    return overlapped_launch(k_fp4_cache_write<TYPE>, dim3((unsigned)grid, count), 256, 0, s, p, slots, token_count, group);
+    if (threads > 0x7fffff00u) return cudaErrorInvalidValue;   // threads and vectors are counted in 31 bits
+    const dim3 grid((unsigned)((threads + 255) / 256), count);
+    if (two) return overlapped_launch(k_fp4_cache_write<TYPE, true>, grid, 256, 0, s, p, slots, token_count);
+    return overlapped_launch(k_fp4_cache_write<TYPE, false>, grid, 256, 0, s, p, slots, token_count);
 }
 template <int TYPE>
 cudaError_t read_impl(const CachePair &p, uint32_t count, const int32_t *table, uint32_t table_width, const int32_t *lengths,
                       uint32_t sequences, uint32_t max_tokens, cudaStream_t s) {
     uint32_t per_token = 0;
-    for (uint32_t i = 0; i < count; ++i) per_token = std::max(per_token, p.cache[i].heads * (p.cache[i].dim / 16));
+    for (uint32_t i = 0; i < count; ++i) per_token = std::max(per_token, p.side[i].cache.heads * p.side[i].blocks.d);
     const uint32_t tokens = std::max(1u, 1024u / per_token);   // about four blocks a thread
     return overlapped_launch(k_fp4_cache_read<TYPE>, dim3((max_tokens + tokens - 1) / tokens, count, sequences), 256, 0, s, p, table,
                              table_width, lengths, max_tokens, tokens);

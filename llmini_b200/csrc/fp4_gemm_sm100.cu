@@ -70,7 +70,7 @@ struct Epilogue {
     uint32_t a_rows, b_rows;   // a scale for every row of A (B)
     uint32_t type;             // of c
     uint32_t accumulate;
-    uint32_t bulk;             // rows of c start on 16-byte boundaries: c has a tensor map
+    uint32_t bulk;             // rows of c start and end on 16-byte boundaries: c has a tensor map
 };
 
 // Sums of 32 columns from `col` on, scaled (s: the scale of A's row, and B's where it has one for all) and biased (`bias`: theirs, in
@@ -776,7 +776,8 @@ Epilogue epilogue_of(const b2_nvfp4_operand &b, const b2_matrix &c, const float 
     epi.b_rows = b.scale_count != 1;
     epi.type = c.type;
     epi.accumulate = accumulate;
-    epi.bulk = reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && epi.pitch % 16 == 0;
+    // a bulk store writes whole 16-byte pieces: where a row's last one is not all its own, the bytes behind the row would change
+    epi.bulk = reinterpret_cast<uintptr_t>(c.data) % 16 == 0 && epi.pitch % 16 == 0 && (uint64_t)c.cols * (c.type == B2_TYPE_F32 ? 4 : 2) % 16 == 0;
     return epi;
 }
 

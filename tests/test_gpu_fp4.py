@@ -184,9 +184,9 @@ def test_matmul(module, m, n, k):
         assert (err <= product_bound(a, b, want, dtype)).all(), (dtype, np.argwhere(~(err <= product_bound(a, b, want, dtype)))[:5])
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512)])
+@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512), (1100, 523, 144), (1100, 790, 64), (40, 67, 48), (130, 1, 16)])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (0, 3), (8, 8)])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (0, 3), (8, 8), (5, 1)])
 def test_matmul_epilogue(module, m, n, k, dtype, offset, pad):
     """Scales for rows of both sides, a bias, rows of c with gaps and starts on every boundary: nothing else of c's memory changes."""
     rng = np.random.default_rng(m * n)
@@ -205,7 +205,7 @@ def test_matmul_epilogue(module, m, n, k, dtype, offset, pad):
     assert (memory == -3.0).all()
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512)])
+@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512), (1100, 523, 144), (1100, 788, 64)])
 @pytest.mark.parametrize("pad", [0, 1])
 def test_matmul_accumulates(module, m, n, k, pad):
     rng = np.random.default_rng(m + 1)

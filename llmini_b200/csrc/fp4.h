@@ -41,10 +41,15 @@ inline cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &d
 
 // ---- fp4_kernels.cu --------------------------------------------------------------------------------------------------
 cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s);
-// Scales on top of parts of x, whose largest is the tensor's: writes `*count` (at most B2_NVFP4_MAXIMA) of them.
-cudaError_t launch_fp4_maxima(const b2_matrix &x, float *maxima, uint32_t *count, int sm_count, cudaStream_t s);
-cudaError_t launch_fp4_quantize_columns(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count,
-                                        int sm_count, cudaStream_t s);
+// One or two tensors by columns.  `tops`: scales on top of parts of x where they are known (those of its rows), else null.
+// maxima: B2_NVFP4_MAXIMA floats a tensor.
+struct ColumnsTask {
+    const b2_matrix *x;
+    const b2_nvfp4_operand *out;
+    const float *tops;
+    uint32_t top_count;
+};
+cudaError_t launch_fp4_quantize_columns(const ColumnsTask *tasks, uint32_t count, float *maxima, int sm_count, cudaStream_t s);
 cudaError_t launch_fp4_decode(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s);
 cudaError_t launch_fp4_cache_write(const b2_nvfp4_cache *caches, const b2_vectors *tokens, uint32_t count, const int64_t *slots,
                                    uint32_t token_count, cudaStream_t s);

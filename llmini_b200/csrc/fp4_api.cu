@@ -7,7 +7,6 @@ namespace {
 
 using b2::launch_fp4_decode;
 using b2::launch_fp4_matmul;
-using b2::launch_fp4_maxima;
 using b2::launch_fp4_quantize_columns;
 using b2::launch_fp4_quantize_rows;
 
@@ -64,10 +63,6 @@ bool good(const b2_nvfp4_cache *caches, const b2_vectors *vectors, uint32_t coun
     return true;
 }
 
-int columns(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count, int sms, cudaStream_t s) {
-    return (int)launch_fp4_quantize_columns(x, out, maxima, count, sms, s);
-}
-
 }  // namespace
 
 extern "C" {
@@ -84,9 +79,8 @@ int b2_nvfp4_quantize_columns(const b2_matrix *x, const b2_nvfp4_operand *out, f
     int sms = 0;
     cudaError_t e = sm_count(sms);
     if (e != cudaSuccess) return (int)e;
-    uint32_t count = 0;
-    e = launch_fp4_maxima(*x, d_maxima, &count, sms, as_stream(stream));
-    return e != cudaSuccess ? (int)e : columns(*x, *out, d_maxima, count, sms, as_stream(stream));
+    const b2::ColumnsTask task = {x, out, nullptr, 0};
+    return (int)launch_fp4_quantize_columns(&task, 1, d_maxima, sms, as_stream(stream));
 }
 
 int b2_nvfp4_decode(const b2_nvfp4_operand *in, uint32_t scale_layout, const b2_matrix *out, void *stream) {
@@ -148,18 +142,9 @@ int b2_nvfp4_linear_backward(const b2_nvfp4_linear_gradients *g, void *stream) {
         if (e == cudaSuccess && g->grad_x.cols != 0) e = launch_fp4_matmul(g->grad_rows, g->weight_t, g->grad_x, nullptr, false, sms, s);
     }
     if (e != cudaSuccess || !to_weight || g->x.cols == 0) return (int)e;
-    uint32_t count = 0;
-    // the rows' scales are scales of parts of the tensor: with them the first pass over grad is done
-    const float *maxima = g->grad_rows.scale;
-    if (to_x) {
-        count = tokens;
-    } else {
-        maxima = g->d_maxima;
-        e = launch_fp4_maxima(g->grad, g->d_maxima, &count, sms, s);
-    }
-    if (e == cudaSuccess) e = (cudaError_t)columns(g->grad, g->grad_columns, maxima, count, sms, s);
-    if (e == cudaSuccess) e = launch_fp4_maxima(g->x, g->d_maxima + B2_NVFP4_MAXIMA, &count, sms, s);
-    if (e == cudaSuccess) e = (cudaError_t)columns(g->x, g->x_columns, g->d_maxima + B2_NVFP4_MAXIMA, count, sms, s);
+    // the scales of grad's rows are scales of parts of it: with them its first pass is done
+    const b2::ColumnsTask tasks[2] = {{&g->grad, &g->grad_columns, to_x ? g->grad_rows.scale : nullptr, tokens}, {&g->x, &g->x_columns, nullptr, 0}};
+    e = launch_fp4_quantize_columns(tasks, 2, g->d_maxima, sms, s);
     if (e == cudaSuccess) e = launch_fp4_matmul(g->grad_columns, g->x_columns, g->grad_weight, nullptr, g->accumulate != 0, sms, s);
     return (int)e;
 }

@@ -793,14 +793,17 @@ cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand 
         const int k = atoi(v);
         if (k == 0 && a.rows <= kFewRows) return few_impl<-1>(&a, nullptr, b, epi, sm_count, s);
         if (k == 1) return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
-        if (k == 2) return gemm_impl<true, 128>(a, b, c, epi, sm_count, s);
         if (k == 3) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
     }
 #endif
     // Few rows: 24 x 1600 -> 50304 takes 8.5 us, in tiles 17.6; 24 x 6400 -> 1600, eight CTAs sharing K, 5.8 and 11.0; 16 x 768 ->
     // 2304 is even (4.1, 3.8).  From 33 rows on only a long K pays: 64 x 6400 -> 1600 7.2 and 11.1, 64 x 1600 -> 4800 7.6 and 5.5.
     if (a.rows <= kFewRows / 2 || (a.rows <= kFewRows && a.cols >= 4096)) return few_impl<-1>(&a, nullptr, b, epi, sm_count, s);
-    if (a.rows >= 1024) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
+    // Tiles of one CTA while every one of them has an SM to itself (777 x 1600 -> 1600 6.0 us, in pairs 7.1; 1000 x 768 -> 2304 4.6
+    // and 5.8), else pairs, which take in half as much for an operation (200 x 1600 -> 50304 20.7 and 14.5; 2000 x 6400 -> 1600 20.4
+    // and 13.0; 512 x 1600 -> 4800, 152 tiles, 8.0 and 7.2).
+    const uint64_t tiles = (uint64_t)((a.rows + 127) / 128) * ((b.rows + 127) / 128);
+    if (tiles > (uint64_t)sm_count) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
     return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
 }
 

@@ -76,64 +76,89 @@ k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t
 }
 
 // ---- by columns -------------------------------------------------------------------------------------------------------------
-// Scales on top of parts of the tensor.  Rows without gaps are one row.
+// Both gradients' operands go through these in one launch: blockIdx.y is the tensor.
+struct MaximaJob {
+    const uint8_t *x;        // rows without gaps are one row
+    uint64_t ld_bytes, cols;
+    uint32_t rows, ctas;
+    const float *tops;       // or what is known already: scales on top of parts of the tensor
+    uint32_t top_count, vec;
+    float *maxima;           // a scale for every CTA's part
+};
+struct MaximaJobs {
+    MaximaJob job[2];
+};
 template <int TYPE>
 __global__ void __launch_bounds__(256, 6)
-k_fp4_maxima(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint64_t cols, bool vec, float *maxima) {
+k_fp4_maxima(const __grid_constant__ MaximaJobs jobs) {
     stream_enter();
     __shared__ uint32_t part[8];
+    const MaximaJob &j = jobs.job[blockIdx.y];
+    if (blockIdx.x >= j.ctas) return;
     uint32_t m = 0;
-    const uint64_t blocks = (cols + 15) / 16;
+    const uint64_t blocks = (j.cols + 15) / 16;
+    const bool vec = j.vec != 0;
     auto take = [&](const uint8_t *src, uint64_t blk) {
         Raw<TYPE> r;
-        r.load(src + blk * 16 * Raw<TYPE>::kSize, cols - blk * 16 < 16 ? (int)(cols - blk * 16) : 16, vec);
+        r.load(src + blk * 16 * Raw<TYPE>::kSize, j.cols - blk * 16 < 16 ? (int)(j.cols - blk * 16) : 16, vec);
         m = max_bits(m, r.amax_bits());
     };
-    if (rows == 1) {
+    if (j.tops) {
+        for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < j.top_count; i += j.ctas * 256) m = max_bits(m, __float_as_uint(j.tops[i]));
+    } else if (j.rows == 1) {
 #pragma unroll 4
-        for (uint64_t blk = blockIdx.x * 256ull + threadIdx.x; blk < blocks; blk += gridDim.x * 256ull) take(x, blk);
+        for (uint64_t blk = blockIdx.x * 256ull + threadIdx.x; blk < blocks; blk += j.ctas * 256ull) take(j.x, blk);
     } else {
-        for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8)
+        for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < j.rows; row += j.ctas * 8)
 #pragma unroll 4
-            for (uint64_t blk = threadIdx.x & 31u; blk < blocks; blk += 32) take(x + (uint64_t)row * ld_bytes, blk);
+            for (uint64_t blk = threadIdx.x & 31u; blk < blocks; blk += 32) take(j.x + (uint64_t)row * j.ld_bytes, blk);
     }
     m = warp_max_bits(m);
     if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) m = max_bits(m, part[i]);
-        maxima[blockIdx.x] = top_scale(m);
+        j.maxima[blockIdx.x] = j.tops ? __uint_as_float(m) : top_scale(m);
     }
 }
 
 // A CTA transposes tiles of 128 rows x 128 columns: a warp takes 16 rows, a lane four columns of them, so that a thread holds
 // four whole blocks of the transpose and their codes only change places on the way to memory, through shared memory.
 constexpr int kTile = 128;
+struct ColumnsJob {
+    const uint8_t *x;
+    uint64_t ld_bytes;
+    uint32_t rows, cols;
+    uint8_t *bytes;
+    uint64_t row_bytes;
+    uint8_t *scales;
+    float *scale;
+    const float *maxima;   // scales on top of parts of the tensor: theirs is the largest
+    uint32_t count, vec;
+};
+struct ColumnsJobs {
+    ColumnsJob job[2];
+};
 template <int TYPE>
 __global__ void __launch_bounds__(256)
-k_fp4_quantize_columns(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t cols, bool vec, uint8_t *bytes, uint64_t row_bytes,
-                       uint8_t *scales, float *scale, const float *maxima, uint32_t count) {
+k_fp4_quantize_columns(const __grid_constant__ ColumnsJobs jobs) {
     stream_enter();
     __shared__ uint2 codes_tile[kTile * 8];   // [column][block of 16 rows], the blocks of a column in an order of its own
     __shared__ __align__(16) uint8_t scales_tile[2 * 512];
     __shared__ uint32_t part[8];
+    const ColumnsJob &job = jobs.job[blockIdx.y];
+    const uint32_t rows = job.rows, cols = job.cols;
+    const uint64_t ld_bytes = job.ld_bytes;
+    const bool vec = job.vec != 0;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    uint32_t m = 0;
-    for (uint32_t i = threadIdx.x; i < count; i += 256) m = max_bits(m, __float_as_uint(maxima[i]));
-    m = warp_max_bits(m);
-    if (lane == 0) part[warp] = m;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_bits(m, part[i]);
-    const float g = __uint_as_float(m), inv = top_inverse(g);
-    if (blockIdx.x == 0 && threadIdx.x == 0) scale[0] = g;
+    float g = 0.0f, inv = 0.0f;
     constexpr int kSize = Raw<TYPE>::kSize;
     const uint32_t blocks = (rows + 15) / 16, chunks = (blocks + 3) / 4;
     const uint32_t tiles_r = (rows + kTile - 1) / kTile, tiles_c = (cols + kTile - 1) / kTile;
     for (uint64_t tile = blockIdx.x; tile < (uint64_t)tiles_r * tiles_c; tile += gridDim.x) {
         const uint32_t tr = (uint32_t)(tile / tiles_c), tc = (uint32_t)(tile % tiles_c);
         const uint32_t r0 = tr * kTile + warp * 16, c0 = tc * kTile + lane * 4;
-        const uint8_t *src = x + (uint64_t)r0 * ld_bytes + (uint64_t)c0 * kSize;
+        const uint8_t *src = job.x + (uint64_t)r0 * ld_bytes + (uint64_t)c0 * kSize;
         // word [i][k]: two values (16-bit) or one (FP32) of row r0 + i
         uint32_t w[16][kSize];
         if (vec && c0 + 4 <= cols) {
@@ -167,6 +192,18 @@ k_fp4_quantize_columns(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint3
                 }
             }
         }
+        if (tile == blockIdx.x) {   // the scale on top, while the first tile is on its way
+            uint32_t m = 0;
+            for (uint32_t i = threadIdx.x; i < job.count; i += 256) m = max_bits(m, __float_as_uint(job.maxima[i]));
+            m = warp_max_bits(m);
+            if (lane == 0) part[warp] = m;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max_bits(m, part[i]);
+            g = __uint_as_float(m);
+            inv = top_inverse(g);
+            if (blockIdx.x == 0 && threadIdx.x == 0) job.scale[0] = g;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             Raw<TYPE> r;   // column c0 + j
@@ -186,11 +223,11 @@ k_fp4_quantize_columns(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint3
         for (int k = 0; k < 4; ++k) {
             const uint32_t c = threadIdx.x / 8 + 32 * k, blk = threadIdx.x & 7u;
             if (tc * kTile + c < cols && tr * 8 + blk < blocks)
-                *reinterpret_cast<uint2 *>(bytes + (uint64_t)(tc * kTile + c) * row_bytes + (uint64_t)(tr * 8 + blk) * 8) =
+                *reinterpret_cast<uint2 *>(job.bytes + (uint64_t)(tc * kTile + c) * job.row_bytes + (uint64_t)(tr * 8 + blk) * 8) =
                     codes_tile[c * 8 + (blk ^ (c >> 2 & 7u))];
         }
         if (threadIdx.x < 64 && tr * 2 + threadIdx.x / 32 < chunks)
-            reinterpret_cast<uint4 *>(scales + ((uint64_t)tc * chunks + tr * 2) * 512)[threadIdx.x] =
+            reinterpret_cast<uint4 *>(job.scales + ((uint64_t)tc * chunks + tr * 2) * 512)[threadIdx.x] =
                 reinterpret_cast<const uint4 *>(scales_tile)[threadIdx.x];
         __syncthreads();
     }
@@ -339,25 +376,45 @@ cudaError_t rows_impl(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStrea
     return go(k_fp4_quantize_rows<TYPE, 16, false>, 1, 512);
 }
 template <int TYPE>
-cudaError_t maxima_impl(const b2_matrix &x, float *maxima, uint32_t *count, int sm_count, cudaStream_t s) {
-    const uint64_t ld = x.ld * Raw<TYPE>::kSize;
-    const bool flat = x.ld == x.cols || x.rows == 1;
-    const uint32_t rows = flat ? 1u : x.rows;
-    const uint64_t cols = flat ? (uint64_t)x.rows * x.cols : x.cols;
-    // the warps' worth of work there is, up to 8 CTAs an SM
-    const uint64_t warps = flat ? (cols + 511) / 512 : rows;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((warps + 7) / 8, std::min(B2_NVFP4_MAXIMA, sm_count * 6));
-    *count = grid;
-    return overlapped_launch(k_fp4_maxima<TYPE>, dim3(grid), 256, 0, s, static_cast<const uint8_t *>(x.data), ld, rows, cols,
-                             aligned(x.data, rows == 1 ? 0 : ld, 16), maxima);
-}
-template <int TYPE>
-cudaError_t columns_impl(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count, int sm_count, cudaStream_t s) {
-    const uint64_t ld = x.ld * Raw<TYPE>::kSize;
-    const uint64_t tiles = (uint64_t)((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(tiles, (uint64_t)sm_count * 4);
-    return overlapped_launch(k_fp4_quantize_columns<TYPE>, dim3(grid), 256, 0, s, static_cast<const uint8_t *>(x.data), ld, x.rows, x.cols,
-                             aligned(x.data, ld, 4 * Raw<TYPE>::kSize), out.bytes, out.row_bytes, out.scales, out.scale, maxima, count);
+cudaError_t columns_impl(const ColumnsTask *tasks, uint32_t count, float *maxima, int sm_count, cudaStream_t s) {
+    MaximaJobs m = {};
+    ColumnsJobs c = {};
+    uint32_t parts = 0, tiles = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+        const b2_matrix &x = *tasks[i].x;
+        const b2_nvfp4_operand &out = *tasks[i].out;
+        const uint64_t ld = x.ld * Raw<TYPE>::kSize;
+        const bool flat = x.ld == x.cols || x.rows == 1;
+        MaximaJob &j = m.job[i];
+        j.x = static_cast<const uint8_t *>(x.data);
+        j.ld_bytes = ld;
+        j.rows = flat ? 1u : x.rows;
+        j.cols = flat ? (uint64_t)x.rows * x.cols : x.cols;
+        j.vec = aligned(x.data, flat ? 0 : ld, 16);
+        j.tops = tasks[i].tops;
+        j.top_count = tasks[i].top_count;
+        j.maxima = maxima + i * B2_NVFP4_MAXIMA;
+        // as many CTAs as there is work for, up to six an SM; a few for scales
+        const uint64_t warps = flat ? (j.cols + 511) / 512 : j.rows, most = std::min(B2_NVFP4_MAXIMA, sm_count * 6);
+        j.ctas = j.tops ? std::min(8u, (j.top_count + 255) / 256) : (uint32_t)std::min((warps + 7) / 8, most);
+        parts = std::max(parts, j.ctas);
+        ColumnsJob &q = c.job[i];
+        q.x = static_cast<const uint8_t *>(x.data);
+        q.ld_bytes = ld;
+        q.rows = x.rows;
+        q.cols = x.cols;
+        q.bytes = out.bytes;
+        q.row_bytes = out.row_bytes;
+        q.scales = out.scales;
+        q.scale = out.scale;
+        q.maxima = j.maxima;
+        q.count = j.ctas;
+        q.vec = aligned(x.data, ld, 4 * Raw<TYPE>::kSize);
+        const uint64_t t = (uint64_t)((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
+        tiles = std::max(tiles, (uint32_t)std::min<uint64_t>(t, 1u << 20));
+    }
+    const cudaError_t e = overlapped_launch(k_fp4_maxima<TYPE>, dim3(parts, count), 256, 0, s, m);
+    return e != cudaSuccess ? e : overlapped_launch(k_fp4_quantize_columns<TYPE>, dim3(tiles, count), 256, 0, s, c);
 }
 template <int TYPE>
 cudaError_t decode_impl(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s) {
@@ -414,12 +471,12 @@ cudaError_t read_impl(const CachePair &p, uint32_t count, const int32_t *table, 
 cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s) {
     B2_FOR_TYPE(x.type, rows_impl, x, out, s)
 }
-cudaError_t launch_fp4_maxima(const b2_matrix &x, float *maxima, uint32_t *count, int sm_count, cudaStream_t s) {
-    B2_FOR_TYPE(x.type, maxima_impl, x, maxima, count, sm_count, s)
-}
-cudaError_t launch_fp4_quantize_columns(const b2_matrix &x, const b2_nvfp4_operand &out, const float *maxima, uint32_t count, int sm_count,
-                                        cudaStream_t s) {
-    B2_FOR_TYPE(x.type, columns_impl, x, out, maxima, count, sm_count, s)
+cudaError_t launch_fp4_quantize_columns(const ColumnsTask *tasks, uint32_t count, float *maxima, int sm_count, cudaStream_t s) {
+    if (count == 2 && tasks[0].x->type != tasks[1].x->type) {
+        const cudaError_t e = launch_fp4_quantize_columns(tasks, 1, maxima, sm_count, s);
+        return e != cudaSuccess ? e : launch_fp4_quantize_columns(tasks + 1, 1, maxima + B2_NVFP4_MAXIMA, sm_count, s);
+    }
+    B2_FOR_TYPE(tasks[0].x->type, columns_impl, tasks, count, maxima, sm_count, s)
 }
 cudaError_t launch_fp4_decode(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s) {
     B2_FOR_TYPE(out.type, decode_impl, in, layout, out, s)

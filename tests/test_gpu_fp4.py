@@ -205,6 +205,37 @@ def test_matmul_epilogue(module, m, n, k, dtype, offset, pad):
     assert (memory == -3.0).all()
 
 
+# rows of c on no boundary in the kernels of both tile shapes; last units of 1, 64, 67, 71, 72, 73, 127 and 128 columns
+ODD_ROWS = [(64, 65), (129, 127), (300, 1031), (161, 200), (257, 455), (33, 521), (1100, 2643), (2049, 2631), (700, 4168), (1000, 4169), (2000, 2751), (2016, 2689)]
+
+
+@pytest.mark.parametrize("m,n", ODD_ROWS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (2, 3), (4, 2), (7, 5), (3, 12)])
+def test_matmul_into_odd_rows(module, m, n, dtype, offset, pad):
+    """Every value of c, in rows that are 0 .. 7 places off a boundary, and nothing between or around them; the same bits twice."""
+    rng = np.random.default_rng(m + n)
+    k = 336 if m < 400 else 80
+    a, oa = operand(rng, m, k, True)
+    b, ob = operand(rng, n, k, False)
+    bias = rng.standard_normal(n).astype(np.float32)
+    a, oa.scale = a / 64, oa.scale.div_(64)
+    outs = []
+    for _ in range(2):
+        memory = torch.full((offset + m * (n + pad) + 64,), -3.0, dtype=TYPES[dtype], device="cuda")
+        c = memory[offset:offset + m * (n + pad)].view(m, n + pad)[:, :n]
+        module.matmul(oa, ob, c, bias=torch.from_numpy(bias).cuda())
+        assert module.status() == 0
+        outs.append(c.clone())
+        c.fill_(-3.0)
+        assert (memory == -3.0).all()
+    want = a @ b.T + bias.astype(np.float64)
+    bound = product_bound(a, b, want, TYPES[dtype]) + np.abs(bias) * 2.0 ** -22
+    wrong = ~(np.abs(plain.to_double(outs[0]) - want) <= bound)
+    assert not wrong.any(), np.argwhere(wrong)[:5]
+    assert torch.equal(outs[0], outs[1])
+
+
 @pytest.mark.parametrize("m,n,k", [(5, 70, 64), (140, 300, 272), (600, 1000, 512), (1100, 523, 144), (1100, 788, 64)])
 @pytest.mark.parametrize("pad", [0, 1])
 def test_matmul_accumulates(module, m, n, k, pad):

@@ -73,15 +73,38 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
 }
 
 // ---- plain values: blocks of 16 -------------------------------------------------------------------------------------------
+// How a thread reaches its block: 32 bytes an instruction (a warp's lanes side by side then move whole lines, where two halves of
+// 16 bytes touch every line twice), 16 bytes, or value by value.
+enum Access : uint32_t { kByValue = 0, kBy16 = 1, kBy32 = 2 };
+__host__ __device__ inline uint32_t access_of(const void *p, uint64_t step_bytes) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(p) | step_bytes;
+    return at % 32 == 0 ? kBy32 : at % 16 == 0 ? kBy16 : kByValue;
+}
+__device__ __forceinline__ void load_32(const uint8_t *p, uint32_t *w) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store_32(uint8_t *p, const uint32_t *w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
 template <int TYPE>
 struct Raw {
     static constexpr int kWords = TYPE == B2_TYPE_F32 ? 16 : 8;
     static constexpr int kSize = TYPE == B2_TYPE_F32 ? 4 : 2;
     uint32_t w[kWords];
 
-    // `n` values (at most 16) from element `p` on, zeros behind them; `vec`: p is on a 16-byte boundary
-    __device__ __forceinline__ void load(const uint8_t *p, int n, bool vec) {
-        if (n >= 16 && vec) {
+    // `n` values (at most 16) from element `p` on, zeros behind them
+    __device__ __forceinline__ void load(const uint8_t *p, int n, uint32_t access) {
+        if (n >= 16 && access == kBy32) {
+#pragma unroll
+            for (int i = 0; i < kWords / 8; ++i) load_32(p + 32 * i, w + 8 * i);
+            return;
+        }
+        if (n >= 16 && access == kBy16) {
 #pragma unroll
             for (int i = 0; i < kWords / 4; ++i) {
                 const uint4 v = *reinterpret_cast<const uint4 *>(p + 16 * i);
@@ -189,29 +212,25 @@ __device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, f
         }
     }
 }
-// `n` values (at most 16) to element `p` on; `vec`: p is on a 16-byte boundary
+// `n` values (at most 16) to element `p` on
 template <int TYPE>
-__device__ __forceinline__ void store_block(uint8_t *p, const float (&v)[16], int n, bool vec) {
-    if (TYPE == B2_TYPE_F32) {
-        if (n >= 16 && vec) {
+__device__ __forceinline__ void store_block(uint8_t *p, const float (&v)[16], int n, uint32_t access) {
+    constexpr int kWords = Raw<TYPE>::kWords;
+    uint32_t w[kWords];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<float4 *>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        } else {
+    for (int i = 0; i < kWords; ++i) w[i] = TYPE == B2_TYPE_F32 ? __float_as_uint(v[i]) : pack_operands(v[2 * i % 16], v[2 * i % 16 + 1], TYPE == B2_TYPE_F16);
+    if (n >= 16 && access == kBy32) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < n) reinterpret_cast<float *>(p)[i] = v[i];
-        }
+        for (int i = 0; i < kWords / 8; ++i) store_32(p + 32 * i, w + 8 * i);
+    } else if (n >= 16 && access == kBy16) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4 *>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     } else {
-        uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = pack_operands(v[2 * i], v[2 * i + 1], TYPE == B2_TYPE_F16);
-        if (n >= 16 && vec) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) reinterpret_cast<uint4 *>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < n) reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        for (int i = 0; i < 16; ++i) {
+            if (i >= n) continue;
+            if (TYPE == B2_TYPE_F32) reinterpret_cast<uint32_t *>(p)[i] = w[i % kWords];
+            else reinterpret_cast<uint16_t *>(p)[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
         }
     }
 }

@@ -584,7 +584,7 @@ struct FewShape {
     // plain values
     const uint8_t *x;
     uint64_t x_pitch;      // bytes
-    uint32_t x_cols, x_vec;
+    uint32_t x_cols, x_access;
 };
 // Shared memory behind the 1024 bytes of barriers and the rows' scales: the pipeline's stages; TYPE >= 0: codes and scales of the
 // rows of A for the CTA's part of K; the sums that the cluster sends.
@@ -711,7 +711,7 @@ k_fp4_few(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         const uint32_t t = threadIdx.x - 64, blocks = shape.K / 16;
         auto load = [&](Raw<T> &r, uint32_t row, uint32_t blk) {
             if (blk * 16 >= shape.x_cols) r.clear();
-            else r.load(shape.x + row * shape.x_pitch + (uint64_t)blk * 16 * Raw<T>::kSize, (int)min(shape.x_cols - blk * 16, 16u), shape.x_vec != 0);
+            else r.load(shape.x + row * shape.x_pitch + (uint64_t)blk * 16 * Raw<T>::kSize, (int)min(shape.x_cols - blk * 16, 16u), shape.x_access);
         };
         for (uint32_t i = t; i < epi.M * blocks; i += kFewThreads - 64) {
             Raw<T> r;
@@ -910,7 +910,7 @@ cudaError_t few_impl(const b2_nvfp4_operand *a, const b2_matrix *x, const b2_nvf
         f.x = static_cast<const uint8_t *>(x->data);
         f.x_pitch = x->ld * Raw<kFused ? TYPE : 0>::kSize;
         f.x_cols = x->cols;
-        f.x_vec = reinterpret_cast<uintptr_t>(x->data) % 16 == 0 && f.x_pitch % 16 == 0;
+        f.x_access = access_of(x->data, f.x_pitch);
     }
     const uint32_t tiles = (b.rows + 127) / 128, all = (b.cols + kStageK - 1) / kStageK;
     f.split = std::max(1u, std::min({kFewSplit, all, (uint32_t)sm_count / tiles}));

@@ -18,7 +18,7 @@ namespace {
 constexpr int kHeld = 4;
 template <int TYPE, int WPR, bool HELD>
 __global__ void __launch_bounds__(WPR == 16 ? 512 : 256)
-k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t cols, bool vec, uint8_t *bytes, uint64_t row_bytes,
+k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t cols, uint32_t access, uint8_t *bytes, uint64_t row_bytes,
                     uint8_t *scales, float *scale) {
     stream_enter();
     constexpr int kWarps = WPR == 16 ? 16 : 8, kRowsPerCta = kWarps / WPR, kThreadsPerRow = 32 * WPR;
@@ -29,7 +29,7 @@ k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t
     const uint32_t blocks = (cols + 15) / 16, tiles = (blocks + 3) / 4;
     const uint8_t *src = x + (uint64_t)row * ld_bytes;
     auto fetch = [&](Raw<TYPE> &r, uint32_t blk) {
-        if (there && blk < blocks) r.load(src + (uint64_t)blk * 16 * Raw<TYPE>::kSize, (int)min(cols - blk * 16u, 16u), vec);
+        if (there && blk < blocks) r.load(src + (uint64_t)blk * 16 * Raw<TYPE>::kSize, (int)min(cols - blk * 16u, 16u), access);
         else r.clear();
     };
     Raw<TYPE> held[HELD ? kHeld : 1];
@@ -82,14 +82,14 @@ struct MaximaJob {
     uint64_t ld_bytes, cols;
     uint32_t rows, ctas;
     const float *tops;       // or what is known already: scales on top of parts of the tensor
-    uint32_t top_count, vec;
+    uint32_t top_count, access;
     float *maxima;           // a scale for every CTA's part
 };
 struct MaximaJobs {
     MaximaJob job[2];
 };
 template <int TYPE>
-__global__ void __launch_bounds__(256, 6)
+__global__ void __launch_bounds__(256, TYPE == B2_TYPE_F32 ? 4 : 6)
 k_fp4_maxima(const __grid_constant__ MaximaJobs jobs) {
     stream_enter();
     __shared__ uint32_t part[8];
@@ -97,10 +97,10 @@ k_fp4_maxima(const __grid_constant__ MaximaJobs jobs) {
     if (blockIdx.x >= j.ctas) return;
     uint32_t m = 0;
     const uint64_t blocks = (j.cols + 15) / 16;
-    const bool vec = j.vec != 0;
+    const uint32_t access = j.access;
     auto take = [&](const uint8_t *src, uint64_t blk) {
         Raw<TYPE> r;
-        r.load(src + blk * 16 * Raw<TYPE>::kSize, j.cols - blk * 16 < 16 ? (int)(j.cols - blk * 16) : 16, vec);
+        r.load(src + blk * 16 * Raw<TYPE>::kSize, j.cols - blk * 16 < 16 ? (int)(j.cols - blk * 16) : 16, access);
         m = max_bits(m, r.amax_bits());
     };
     if (j.tops) {
@@ -237,7 +237,7 @@ k_fp4_quantize_columns(const __grid_constant__ ColumnsJobs jobs) {
 template <int TYPE>
 __global__ void __launch_bounds__(256)
 k_fp4_decode(const uint8_t *bytes, uint64_t row_bytes, const uint8_t *scales, uint32_t layout, const float *scale, bool per_row,
-             uint32_t rows, uint32_t blocks, uint32_t threads_per_row, uint8_t *out, uint64_t ld_bytes, uint32_t cols, bool vec) {
+             uint32_t rows, uint32_t blocks, uint32_t threads_per_row, uint8_t *out, uint64_t ld_bytes, uint32_t cols, uint32_t access) {
     stream_enter();
     const uint32_t row = blockIdx.x * (256u / threads_per_row) + threadIdx.x / threads_per_row;
     if (row >= rows) return;
@@ -250,7 +250,7 @@ k_fp4_decode(const uint8_t *bytes, uint64_t row_bytes, const uint8_t *scales, ui
                            : layout == B2_SCALES_RAW ? scales[flat] : csf_load_scale(scales, (uint32_t)flat);
         float v[16];
         decode_block(codes, s, g, v);
-        store_block<TYPE>(out + (uint64_t)row * ld_bytes + (uint64_t)blk * 16 * Raw<TYPE>::kSize, v, (int)min(cols - blk * 16u, 16u), vec);
+        store_block<TYPE>(out + (uint64_t)row * ld_bytes + (uint64_t)blk * 16 * Raw<TYPE>::kSize, v, (int)min(cols - blk * 16u, 16u), access);
     }
 }
 
@@ -272,7 +272,7 @@ struct CacheSide {
     b2_vectors vectors;
     Divisor heads, blocks;
     uint32_t group;   // lanes of a vector when it is written
-    bool vec;
+    uint32_t access;
 };
 struct CachePair {
     CacheSide side[2];
@@ -297,7 +297,7 @@ k_fp4_cache_write(const __grid_constant__ CachePair p, const int64_t *slots, uin
 #pragma unroll
     for (int i = 0; i < (TWO ? 2 : 1); ++i) {
         const uint32_t blk = lane + i * group;
-        if (there && blk < blocks) r[i].load(src + blk * 16 * Raw<TYPE>::kSize, 16, side.vec);
+        if (there && blk < blocks) r[i].load(src + blk * 16 * Raw<TYPE>::kSize, 16, side.access);
         else r[i].clear();
         m = max_bits(m, r[i].amax_bits());
     }
@@ -349,7 +349,7 @@ k_fp4_cache_read(const __grid_constant__ CachePair p, const int32_t *table, uint
         }
         float v[16];
         decode_block(codes, s, e == 255u ? __uint_as_float(0x7fffffffu) : e == 0u ? 0x1p-127f : __uint_as_float(e << 23), v);
-        store_block<TYPE>(out + (t * side.vectors.token_stride + head * side.vectors.head_stride + blk * 16) * Raw<TYPE>::kSize, v, 16, side.vec);
+        store_block<TYPE>(out + (t * side.vectors.token_stride + head * side.vectors.head_stride + blk * 16) * Raw<TYPE>::kSize, v, 16, side.access);
     }
 }
 
@@ -364,11 +364,11 @@ bool aligned(const void *p, uint64_t step_bytes, uint64_t to) { return reinterpr
 template <int TYPE>
 cudaError_t rows_impl(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s) {
     const uint64_t ld = x.ld * Raw<TYPE>::kSize;
-    const bool vec = aligned(x.data, ld, 16);
+    const uint32_t access = access_of(x.data, ld);
     const uint32_t blocks = out.cols / 16;
     auto go = [&](auto kernel, uint32_t rows_per_cta, int threads) {
         return overlapped_launch(kernel, dim3((x.rows + rows_per_cta - 1) / rows_per_cta), threads, 0, s, static_cast<const uint8_t *>(x.data),
-                                 ld, x.rows, x.cols, vec, out.bytes, out.row_bytes, out.scales, out.scale);
+                                 ld, x.rows, x.cols, access, out.bytes, out.row_bytes, out.scales, out.scale);
     };
     if (blocks <= 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 1, true>, 8, 256);
     if (blocks <= 4 * 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 4, true>, 2, 256);
@@ -390,7 +390,7 @@ cudaError_t columns_impl(const ColumnsTask *tasks, uint32_t count, float *maxima
         j.ld_bytes = ld;
         j.rows = flat ? 1u : x.rows;
         j.cols = flat ? (uint64_t)x.rows * x.cols : x.cols;
-        j.vec = aligned(x.data, flat ? 0 : ld, 16);
+        j.access = access_of(x.data, flat ? 0 : ld);
         j.tops = tasks[i].tops;
         j.top_count = tasks[i].top_count;
         j.maxima = maxima + i * B2_NVFP4_MAXIMA;
@@ -425,7 +425,7 @@ cudaError_t decode_impl(const b2_nvfp4_operand &in, uint32_t layout, const b2_ma
     const uint32_t per_cta = 256 / tpr;
     return overlapped_launch(k_fp4_decode<TYPE>, dim3((in.rows + per_cta - 1) / per_cta), 256, 0, s, static_cast<const uint8_t *>(in.bytes),
                              in.row_bytes, static_cast<const uint8_t *>(in.scales), layout, static_cast<const float *>(in.scale),
-                             in.scale_count != 1, in.rows, blocks, tpr, static_cast<uint8_t *>(out.data), ld, out.cols, aligned(out.data, ld, 16));
+                             in.scale_count != 1, in.rows, blocks, tpr, static_cast<uint8_t *>(out.data), ld, out.cols, access_of(out.data, ld));
 }
 CachePair cache_pair(const b2_nvfp4_cache *caches, const b2_vectors *vectors, uint32_t count) {
     CachePair p = {};
@@ -439,7 +439,7 @@ CachePair cache_pair(const b2_nvfp4_cache *caches, const b2_vectors *vectors, ui
         for (side.group = 1; side.group < side.blocks.d && side.group < 32;) side.group *= 2;
         const uint64_t size = type_size(vectors[i].type);
         const uint64_t strides = (vectors[i].sequence_stride | vectors[i].token_stride | vectors[i].head_stride) * size;
-        side.vec = aligned(vectors[i].data, strides, 16);
+        side.access = access_of(vectors[i].data, strides);
     }
     return p;
 }

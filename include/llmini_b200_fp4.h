@@ -68,8 +68,9 @@ int b2_nvfp4_decode(const b2_nvfp4_operand *in, uint32_t scale_layout, const b2_
 int b2_nvfp4_matmul(const b2_nvfp4_operand *a, const b2_nvfp4_operand *b, const b2_matrix *c, const float *d_bias,
                     uint32_t accumulate, void *stream);
 
-/* y = Q(x) W^T + bias: x [tokens][inputs] quantised by rows into `scratch` (an operand of tokens rows, scale_count = rows),
- * W [outputs][inputs] as it is. */
+/* y = Q(x) W^T + bias: x [tokens][inputs] quantised by rows, W [outputs][inputs] as it is.  `scratch`: memory for Q(x), an operand of
+ * tokens rows, scale_count = rows; a few values are quantised on the way and do not go there, so what it holds afterwards is not
+ * defined. */
 int b2_nvfp4_linear_forward(const b2_matrix *x, const b2_nvfp4_operand *weight, const b2_matrix *y, const float *d_bias,
                             const b2_nvfp4_operand *scratch, void *stream);
 /* The gradients of that, straight through the rounding:

@@ -127,6 +127,13 @@ def _up(n: int, step: int) -> int:
     return -(-n // step) * step
 
 
+def _assign(o, name: str, value) -> None:
+    """Another tensor for a field of an object that calls have the addresses of: they are taken anew."""
+    object.__setattr__(o, name, value)
+    if name in o.__dataclass_fields__ and name != "c" and "device_index" in o.__dict__:
+        o.__post_init__()
+
+
 @dataclass
 class Nvfp4Operand:
     """A matrix in NVFP4 as the product reads it: codes [rows, row_bytes] (two a byte, k / 2 of a row's bytes), block scales in the
@@ -157,6 +164,9 @@ class Nvfp4Operand:
         self.device_index = b.device.index
         self.c = Operand(b.data_ptr(), self.scales.data_ptr(), self.scale.data_ptr(), row_bytes, self.rows, self.k, n, 0)
         self.ref = C.byref(self.c)
+
+    def __setattr__(self, name, value):
+        _assign(self, name, value)
 
     @staticmethod
     def empty(rows: int, k: int, per_row: bool = True, device="cuda") -> "Nvfp4Operand":
@@ -212,6 +222,9 @@ class Nvfp4PagedCache:
         self.sizes = [(s[0].shape[2], s[0].shape[3] * 2) for s in sides]
         self.vectors = Vectors * len(sides)
 
+    def __setattr__(self, name, value):
+        _assign(self, name, value)
+
     @staticmethod
     def empty(pages: int, page_size: int, heads: int, dim: int, value_dim: int | None = None, device="cuda") -> "Nvfp4PagedCache":
         def side(d):
@@ -243,8 +256,8 @@ class Nvfp4LinearModule:
             if (t.k // 2) % 16 and t.rows > 1:
                 _refuse("rows of k values start on 16-byte boundaries where k is a multiple of 32")
             need = _up(t.rows, 128) * _up(t.k // 16, 4) if layout == SCALES_SM100 else t.rows * t.k // 16 if layout == SCALES_RAW else _csf_bytes(t.rows, t.k)
-            if t.bytes.numel() < t.rows * t.k // 2 or t.scales.numel() < need:
-                _refuse("an Nvfp4Tensor with too little memory for its rows and k")
+            if t.bytes.numel() < t.rows * t.k // 2 or t.scales.numel() < need or not (t.bytes.is_contiguous() and t.scales.is_contiguous()):
+                _refuse("an Nvfp4Tensor with too little memory for its rows and k, or with gaps in it")
             c = C.byref(Operand(_here(t.bytes, d), _here(t.scales, d), _here(t.global_scale, d), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
         else:
             c, layout = _operand(operand, d), SCALES_SM100
@@ -305,6 +318,8 @@ class Nvfp4LinearModule:
             t, shape, stride = tensors[i], tensors[i].shape, tensors[i].stride()
             if shape[-2:] != cache.sizes[i] or stride[-1] != 1:
                 _refuse("vectors of the cache's heads and size, their values side by side")
+            if dims == 4 and any(n > 1 and s == 0 for n, s in zip(shape, stride)):
+                _refuse("vectors that are written lie apart")
             if i and (t.dtype != first.dtype or shape[:-2] != first.shape[:-2]):
                 _refuse("keys and values: tensors of one type and length")
             v[i] = Vectors(_here(t, d), stride[0] if dims == 4 else 0, stride[-3], stride[-2], kind, 0)

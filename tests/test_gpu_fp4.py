@@ -588,3 +588,37 @@ def test_refusals(module):
     module.matmul(o(0, 32), o(5, 32), f(0, 5))
     module.matmul(o(4, 32), o(0, 32, per_row=False), f(4, 0))
     module.cache_write(cache, slots[:0], f(0, 3, 32), f(0, 3, 32))
+
+
+def test_fields_may_be_replaced(module):
+    """Calls see the tensors that an operand and a cache have now, not those that they were made with."""
+    x = torch.randn(40, 64, device="cuda")
+    o = b2.Nvfp4Operand.empty(40, 64)
+    first = o.bytes
+    first.fill_(0x55)
+    o.bytes, o.scale = torch.zeros(40, 48, dtype=torch.uint8, device="cuda"), torch.zeros(40, device="cuda")
+    module.quantize_rows(x, o)
+    assert (first == 0x55).all() and o.scale.all()
+    assert (o.bytes[:, 32:] == 0).all() and o.bytes.any()
+    with pytest.raises(ValueError):
+        o.bytes = torch.zeros(39, 32, dtype=torch.uint8, device="cuda")
+    cache, other = (b2.Nvfp4PagedCache.empty(4, 8, 2, 32) for _ in range(2))
+    before = cache.key
+    cache.key = other.key
+    key = torch.randn(3, 2, 32, device="cuda")
+    module.cache_write(cache, torch.arange(3, device="cuda"), key, key)
+    assert not before[0].any() and other.key[0].any() and cache.value[0].any()
+
+
+def test_results_do_not_overlap(module):
+    cache = b2.Nvfp4PagedCache.empty(4, 8, 2, 32)
+    table, lengths = torch.zeros(3, 4, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    good = torch.zeros(3, 8, 2, 32, device="cuda")
+    for bad in (good[:1].expand(3, 8, 2, 32), good[:, :1].expand(3, 8, 2, 32), good[:, :, :1].expand(3, 8, 2, 32)):
+        with pytest.raises(ValueError):
+            module.cache_read(cache, table, lengths, bad, good)
+    # what is read may: one vector for every head and token
+    one = torch.randn(1, 1, 32, device="cuda").expand(5, 2, 32)
+    module.cache_write(cache, torch.arange(5, device="cuda"), one, one)
+    module.cache_read(cache, table, torch.full_like(lengths, 5), good, good.clone())
+    assert torch.equal(good[0, :5], good[1, :5]) and (good[0, :5] == good[0, 0, 0]).all() and good[0, 0, 0].any()

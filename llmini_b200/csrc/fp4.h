@@ -41,8 +41,14 @@ inline cudaError_t allow_smem(K kernel, uint32_t bytes, std::atomic<uint64_t> &d
 
 // ---- fp4_kernels.cu --------------------------------------------------------------------------------------------------
 cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s);
+// The same, and in the same launch the maximum of `other`, of x's type: scales on top of its fp4_maximum_parts(other) parts.
+cudaError_t launch_fp4_quantize_rows_and_maximum(const b2_matrix &x, const b2_nvfp4_operand &out, const b2_matrix &other, float *maxima,
+                                                 int sm_count, cudaStream_t s);
+uint32_t fp4_maximum_parts(const b2_matrix &x, int sm_count);
+// Scales on top of parts of a tensor that every CTA of the columns' kernel goes through for itself; more have a launch of their own.
+constexpr uint32_t kFewTops = 4096;
 // One or two tensors by columns.  `tops`: scales on top of parts of x where they are known (those of its rows), else null.
-// maxima: B2_NVFP4_MAXIMA floats a tensor.
+// maxima: B2_NVFP4_MAXIMA floats a tensor; `tops` may lie there only if there are no more of them.
 struct ColumnsTask {
     const b2_matrix *x;
     const b2_nvfp4_operand *out;

@@ -137,13 +137,20 @@ int b2_nvfp4_linear_backward(const b2_nvfp4_linear_gradients *g, void *stream) {
     }
     int sms = 0;
     cudaError_t e = sm_count(sms);
+    const bool columns = to_weight && g->x.cols != 0;
+    // x's maximum comes along with the rows of grad, which saves a launch where grad's needs none: 777 x 1600 -> 1600 25.9 -> 24.1 us,
+    // 64 x 1024 -> 1024 15.0 -> 13.3; with 8192 rows 85.9 -> 86.8
+    const bool along = to_x && columns && g->x.type == g->grad.type && tokens <= b2::kFewTops;
+    float *x_maxima = along ? g->d_maxima + B2_NVFP4_MAXIMA : nullptr;
     if (e == cudaSuccess && to_x) {
-        e = launch_fp4_quantize_rows(g->grad, g->grad_rows, s);
+        e = along ? b2::launch_fp4_quantize_rows_and_maximum(g->grad, g->grad_rows, g->x, x_maxima, sms, s)
+                  : launch_fp4_quantize_rows(g->grad, g->grad_rows, s);
         if (e == cudaSuccess && g->grad_x.cols != 0) e = launch_fp4_matmul(g->grad_rows, g->weight_t, g->grad_x, nullptr, false, sms, s);
     }
-    if (e != cudaSuccess || !to_weight || g->x.cols == 0) return (int)e;
+    if (e != cudaSuccess || !columns) return (int)e;
     // the scales of grad's rows are scales of parts of it: with them its first pass is done
-    const b2::ColumnsTask tasks[2] = {{&g->grad, &g->grad_columns, to_x ? g->grad_rows.scale : nullptr, tokens}, {&g->x, &g->x_columns, nullptr, 0}};
+    const b2::ColumnsTask tasks[2] = {{&g->grad, &g->grad_columns, to_x ? g->grad_rows.scale : nullptr, tokens},
+                                      {&g->x, &g->x_columns, x_maxima, along ? b2::fp4_maximum_parts(g->x, sms) : 0}};
     e = launch_fp4_quantize_columns(tasks, 2, g->d_maxima, sms, s);
     if (e == cudaSuccess) e = launch_fp4_matmul(g->grad_columns, g->x_columns, g->grad_weight, nullptr, g->accumulate != 0, sms, s);
     return (int)e;

@@ -12,15 +12,60 @@ namespace b2 {
 
 namespace {
 
+// ---- a tensor's maximum -----------------------------------------------------------------------------------------------------
+struct MaximaJob {
+    const uint8_t *x;        // rows without gaps are one row
+    uint64_t ld_bytes, cols;
+    uint32_t rows, ctas;
+    const float *tops;       // or what is known already: scales on top of parts of the tensor
+    uint32_t top_count, access;
+    float *maxima;           // a scale for every CTA's part
+};
+// Part `cta` of job.ctas, in CTAs of 256 threads or 512.
+template <int TYPE>
+__device__ __forceinline__ void part_of_maximum(const MaximaJob &j, uint32_t cta) {
+    __shared__ uint32_t part[16];
+    const uint32_t threads = blockDim.x, warps = threads / 32;
+    uint32_t m = 0;
+    const uint64_t blocks = (j.cols + 15) / 16;
+    const uint32_t access = j.access;
+    auto take = [&](const uint8_t *src, uint64_t blk) {
+        Raw<TYPE> r;
+        r.load(src + blk * 16 * Raw<TYPE>::kSize, j.cols - blk * 16 < 16 ? (int)(j.cols - blk * 16) : 16, access);
+        m = max_bits(m, r.amax_bits());
+    };
+    if (j.tops) {
+        for (uint32_t i = cta * threads + threadIdx.x; i < j.top_count; i += j.ctas * threads) m = max_bits(m, __float_as_uint(j.tops[i]));
+    } else if (j.rows == 1) {
+#pragma unroll 4
+        for (uint64_t blk = cta * (uint64_t)threads + threadIdx.x; blk < blocks; blk += j.ctas * (uint64_t)threads) take(j.x, blk);
+    } else {
+        for (uint32_t row = cta * warps + (threadIdx.x >> 5); row < j.rows; row += j.ctas * warps)
+#pragma unroll 4
+            for (uint64_t blk = threadIdx.x & 31u; blk < blocks; blk += 32) take(j.x + (uint64_t)row * j.ld_bytes, blk);
+    }
+    m = warp_max_bits(m);
+    if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < warps; ++i) m = max_bits(m, part[i]);
+        j.maxima[cta] = j.tops ? __uint_as_float(m) : top_scale(m);
+    }
+}
+
 // ---- by rows ----------------------------------------------------------------------------------------------------------------
 // WPR warps a row; a thread holds kHeld blocks of it, so a row of up to WPR * 32 * kHeld blocks is read once.  A longer one
-// (HELD false) is read twice, the second time out of L2 where it fits.
+// (HELD false) is read twice, the second time out of L2 where it fits.  CTAs behind row_ctas take the maximum of another tensor.
 constexpr int kHeld = 4;
 template <int TYPE, int WPR, bool HELD>
 __global__ void __launch_bounds__(WPR == 16 ? 512 : 256)
 k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t cols, uint32_t access, uint8_t *bytes, uint64_t row_bytes,
-                    uint8_t *scales, float *scale) {
+                    uint8_t *scales, float *scale, uint32_t row_ctas, const __grid_constant__ MaximaJob other) {
     stream_enter();
+    if (blockIdx.x >= row_ctas) {
+        part_of_maximum<TYPE>(other, blockIdx.x - row_ctas);
+        return;
+    }
     constexpr int kWarps = WPR == 16 ? 16 : 8, kRowsPerCta = kWarps / WPR, kThreadsPerRow = 32 * WPR;
     __shared__ uint32_t part[kWarps];
     const uint32_t warp = threadIdx.x >> 5, in_row = threadIdx.x % kThreadsPerRow;
@@ -77,14 +122,6 @@ k_fp4_quantize_rows(const uint8_t *x, uint64_t ld_bytes, uint32_t rows, uint32_t
 
 // ---- by columns -------------------------------------------------------------------------------------------------------------
 // Both gradients' operands go through these in one launch: blockIdx.y is the tensor.
-struct MaximaJob {
-    const uint8_t *x;        // rows without gaps are one row
-    uint64_t ld_bytes, cols;
-    uint32_t rows, ctas;
-    const float *tops;       // or what is known already: scales on top of parts of the tensor
-    uint32_t top_count, access;
-    float *maxima;           // a scale for every CTA's part
-};
 struct MaximaJobs {
     MaximaJob job[2];
 };
@@ -92,34 +129,7 @@ template <int TYPE>
 __global__ void __launch_bounds__(256, TYPE == B2_TYPE_F32 ? 4 : 6)
 k_fp4_maxima(const __grid_constant__ MaximaJobs jobs) {
     stream_enter();
-    __shared__ uint32_t part[8];
-    const MaximaJob &j = jobs.job[blockIdx.y];
-    if (blockIdx.x >= j.ctas) return;
-    uint32_t m = 0;
-    const uint64_t blocks = (j.cols + 15) / 16;
-    const uint32_t access = j.access;
-    auto take = [&](const uint8_t *src, uint64_t blk) {
-        Raw<TYPE> r;
-        r.load(src + blk * 16 * Raw<TYPE>::kSize, j.cols - blk * 16 < 16 ? (int)(j.cols - blk * 16) : 16, access);
-        m = max_bits(m, r.amax_bits());
-    };
-    if (j.tops) {
-        for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < j.top_count; i += j.ctas * 256) m = max_bits(m, __float_as_uint(j.tops[i]));
-    } else if (j.rows == 1) {
-#pragma unroll 4
-        for (uint64_t blk = blockIdx.x * 256ull + threadIdx.x; blk < blocks; blk += j.ctas * 256ull) take(j.x, blk);
-    } else {
-        for (uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5); row < j.rows; row += j.ctas * 8)
-#pragma unroll 4
-            for (uint64_t blk = threadIdx.x & 31u; blk < blocks; blk += 32) take(j.x + (uint64_t)row * j.ld_bytes, blk);
-    }
-    m = warp_max_bits(m);
-    if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) m = max_bits(m, part[i]);
-        j.maxima[blockIdx.x] = j.tops ? __uint_as_float(m) : top_scale(m);
-    }
+    if (blockIdx.x < jobs.job[blockIdx.y].ctas) part_of_maximum<TYPE>(jobs.job[blockIdx.y], blockIdx.x);
 }
 
 // A CTA transposes tiles of 128 rows x 128 columns: a warp takes 16 rows, a lane four columns of them, so that a thread holds
@@ -361,14 +371,30 @@ bool aligned(const void *p, uint64_t step_bytes, uint64_t to) { return reinterpr
     if ((type) == B2_TYPE_BF16) return F<B2_TYPE_BF16>(__VA_ARGS__);   \
     return F<B2_TYPE_F16>(__VA_ARGS__);
 
+// The maximum of x, in as many CTAs as there is work for, up to six an SM; `maxima`: a scale of each.
+MaximaJob maximum_of(const b2_matrix &x, float *maxima, int sm_count) {
+    const uint64_t ld = x.ld * type_size(x.type);
+    const bool flat = x.ld == x.cols || x.rows == 1;
+    MaximaJob j = {};
+    j.x = static_cast<const uint8_t *>(x.data);
+    j.ld_bytes = ld;
+    j.rows = flat ? 1u : x.rows;
+    j.cols = flat ? (uint64_t)x.rows * x.cols : x.cols;
+    j.access = access_of(x.data, flat ? 0 : ld);
+    const uint64_t warps = flat ? (j.cols + 511) / 512 : j.rows, most = std::min(B2_NVFP4_MAXIMA, sm_count * 6);
+    j.ctas = (uint32_t)std::min((warps + 7) / 8, most);
+    j.maxima = maxima;
+    return j;
+}
 template <int TYPE>
-cudaError_t rows_impl(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s) {
+cudaError_t rows_impl(const b2_matrix &x, const b2_nvfp4_operand &out, const MaximaJob &other, cudaStream_t s) {
     const uint64_t ld = x.ld * Raw<TYPE>::kSize;
     const uint32_t access = access_of(x.data, ld);
     const uint32_t blocks = out.cols / 16;
     auto go = [&](auto kernel, uint32_t rows_per_cta, int threads) {
-        return overlapped_launch(kernel, dim3((x.rows + rows_per_cta - 1) / rows_per_cta), threads, 0, s, static_cast<const uint8_t *>(x.data),
-                                 ld, x.rows, x.cols, access, out.bytes, out.row_bytes, out.scales, out.scale);
+        const uint32_t ctas = (x.rows + rows_per_cta - 1) / rows_per_cta;
+        return overlapped_launch(kernel, dim3(ctas + other.ctas), threads, 0, s, static_cast<const uint8_t *>(x.data), ld, x.rows, x.cols, access,
+                                 out.bytes, out.row_bytes, out.scales, out.scale, ctas, other);
     };
     if (blocks <= 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 1, true>, 8, 256);
     if (blocks <= 4 * 32 * kHeld) return go(k_fp4_quantize_rows<TYPE, 4, true>, 2, 256);
@@ -384,19 +410,14 @@ cudaError_t columns_impl(const ColumnsTask *tasks, uint32_t count, float *maxima
         const b2_matrix &x = *tasks[i].x;
         const b2_nvfp4_operand &out = *tasks[i].out;
         const uint64_t ld = x.ld * Raw<TYPE>::kSize;
-        const bool flat = x.ld == x.cols || x.rows == 1;
         MaximaJob &j = m.job[i];
-        j.x = static_cast<const uint8_t *>(x.data);
-        j.ld_bytes = ld;
-        j.rows = flat ? 1u : x.rows;
-        j.cols = flat ? (uint64_t)x.rows * x.cols : x.cols;
-        j.access = access_of(x.data, flat ? 0 : ld);
-        j.tops = tasks[i].tops;
-        j.top_count = tasks[i].top_count;
-        j.maxima = maxima + i * B2_NVFP4_MAXIMA;
-        // as many CTAs as there is work for, up to six an SM; a few for scales
-        const uint64_t warps = flat ? (j.cols + 511) / 512 : j.rows, most = std::min(B2_NVFP4_MAXIMA, sm_count * 6);
-        j.ctas = j.tops ? std::min(8u, (j.top_count + 255) / 256) : (uint32_t)std::min((warps + 7) / 8, most);
+        j = maximum_of(x, maxima + i * B2_NVFP4_MAXIMA, sm_count);
+        const bool few = tasks[i].tops && tasks[i].top_count <= kFewTops;
+        if (tasks[i].tops) {
+            j.tops = tasks[i].tops;
+            j.top_count = tasks[i].top_count;
+            j.ctas = few ? 0 : 8;
+        }
         parts = std::max(parts, j.ctas);
         ColumnsJob &q = c.job[i];
         q.x = static_cast<const uint8_t *>(x.data);
@@ -407,14 +428,17 @@ cudaError_t columns_impl(const ColumnsTask *tasks, uint32_t count, float *maxima
         q.row_bytes = out.row_bytes;
         q.scales = out.scales;
         q.scale = out.scale;
-        q.maxima = j.maxima;
-        q.count = j.ctas;
+        q.maxima = few ? tasks[i].tops : j.maxima;
+        q.count = few ? tasks[i].top_count : j.ctas;
         q.vec = aligned(x.data, ld, 4 * Raw<TYPE>::kSize);
         const uint64_t t = (uint64_t)((x.rows + kTile - 1) / kTile) * ((x.cols + kTile - 1) / kTile);
         tiles = std::max(tiles, (uint32_t)std::min<uint64_t>(t, 1u << 20));
     }
-    const cudaError_t e = overlapped_launch(k_fp4_maxima<TYPE>, dim3(parts, count), 256, 0, s, m);
-    return e != cudaSuccess ? e : overlapped_launch(k_fp4_quantize_columns<TYPE>, dim3(tiles, count), 256, 0, s, c);
+    if (parts != 0) {
+        const cudaError_t e = overlapped_launch(k_fp4_maxima<TYPE>, dim3(parts, count), 256, 0, s, m);
+        if (e != cudaSuccess) return e;
+    }
+    return overlapped_launch(k_fp4_quantize_columns<TYPE>, dim3(tiles, count), 256, 0, s, c);
 }
 template <int TYPE>
 cudaError_t decode_impl(const b2_nvfp4_operand &in, uint32_t layout, const b2_matrix &out, cudaStream_t s) {
@@ -469,7 +493,14 @@ cudaError_t read_impl(const CachePair &p, uint32_t count, const int32_t *table, 
 }  // namespace
 
 cudaError_t launch_fp4_quantize_rows(const b2_matrix &x, const b2_nvfp4_operand &out, cudaStream_t s) {
-    B2_FOR_TYPE(x.type, rows_impl, x, out, s)
+    const MaximaJob none = {};
+    B2_FOR_TYPE(x.type, rows_impl, x, out, none, s)
+}
+uint32_t fp4_maximum_parts(const b2_matrix &x, int sm_count) { return maximum_of(x, nullptr, sm_count).ctas; }
+cudaError_t launch_fp4_quantize_rows_and_maximum(const b2_matrix &x, const b2_nvfp4_operand &out, const b2_matrix &other, float *maxima,
+                                                 int sm_count, cudaStream_t s) {
+    const MaximaJob job = maximum_of(other, maxima, sm_count);
+    B2_FOR_TYPE(x.type, rows_impl, x, out, job, s)
 }
 cudaError_t launch_fp4_quantize_columns(const ColumnsTask *tasks, uint32_t count, float *maxima, int sm_count, cudaStream_t s) {
     if (count == 2 && tasks[0].x->type != tasks[1].x->type) {

@@ -334,6 +334,32 @@ def test_linear_backward(module, tokens, inputs, outputs, dtype):
             within(grad_w, gc, xc, torch.float32, start.astype(np.float64) if accumulate else 0.0)
 
 
+@pytest.mark.parametrize("tokens,inputs,outputs", [(20, 48, 9000), (3, 64, 33008), (5000, 48, 64), (4096, 80, 2064), (4097, 1600, 32), (600, 5000, 16)])
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("gap", [0, 5])
+def test_linear_backward_is_its_parts(module, tokens, inputs, outputs, types, gap):
+    """Bit for bit what the quantisers and the product give one by one: rows of every length, many and few of them, with gaps."""
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    x = torch.randn(tokens, inputs + gap, device="cuda", generator=gen).to(TYPES[types[0]])[:, :inputs]
+    grad = torch.randn(tokens, outputs + gap, device="cuda", generator=gen).to(TYPES[types[1]])[:, :outputs]
+    x[tokens // 2, inputs // 3] = 100.0       # the maxima, each in one place
+    grad[tokens - 1, outputs - 1] = -70.0
+    wt = b2.Nvfp4Operand.empty(inputs, outputs)
+    module.quantize_rows(torch.randn(inputs, outputs, device="cuda", generator=gen), wt)
+    got = torch.empty(tokens, inputs, device="cuda"), torch.empty(outputs, inputs, device="cuda")
+    module.linear_backward(grad, x, wt, *got, b2.Nvfp4LinearScratch(tokens, inputs, outputs, backward=True))
+    maxima = torch.empty(b2.NVFP4_MAXIMA, device="cuda")
+    rows, columns, x_columns = (b2.Nvfp4Operand.empty(r, k, per_row=p) for r, k, p in ((tokens, outputs, True), (outputs, tokens, False), (inputs, tokens, False)))
+    module.quantize_rows(grad, rows)
+    module.quantize_columns(grad, columns, maxima)
+    module.quantize_columns(x, x_columns, maxima)
+    assert x_columns.scale.item() == 2.0 ** (6 - 10) and columns.scale.item() == 2.0 ** (6 - 10)
+    want = torch.empty_like(got[0]), torch.empty_like(got[1])
+    module.matmul(rows, wt, want[0])
+    module.matmul(columns, x_columns, want[1])
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_linear_gradients_are_those_of_the_layer(module):
     """Against differences of sum(grad * (x W^T)): the gradients are off by what the rounding of their operands to 4 bits is.  A
     block's values are off by half a step of E2M1, 1/2 of values 4 .. 6 down to 1/4 of those below 2, in units of max / 6; normal

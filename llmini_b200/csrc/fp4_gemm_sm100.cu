@@ -4,6 +4,12 @@
 //
 // The operands' rows are 128-byte swizzled panels as in the Newton-Schulz GEMM (ns_gemm_sm100.cu): 128 bytes are 256 values of K,
 // four MMAs.  The block scales of 128 rows and 64 values of K are a 512-byte tile, stored as the copy wants it.
+//
+// What bounds it.  8192^3: the MMAs, 5.8 PFLOP/s (190 us).  Short sums: the way between L2 and the SMs.  16384 x 1600 -> 6400 in BF16, 90
+// us, moves 1.18 GB through L2 (13 TB/s), loads of tiles and stores of results together; without its stores it takes 64 us, without
+// its MMAs 80, without the copies of scales 89.  The same for results stored by row, by threads from shared memory or straight from
+// registers in 32-byte pieces (129, 88, 87), for tiles in the other order and for cache hints.  Tiles of 256 x 192, whose
+// accumulators share no columns of tensor memory, load more for a result: 108.
 #include <algorithm>
 #include <atomic>
 #include <cstdlib>

@@ -1,7 +1,11 @@
 // Quantisation of activations and gradients to NVFP4 by rows and by columns, reading 4-bit tensors back, and the paged cache.
-// All of it streams: what bounds these kernels is the way to memory and back.
+// All of it streams: the bytes bound these kernels from below, and at 220 instructions a block the quantisers' arithmetic is about as
+// long, so they issue in 60 to 70 % of the cycles.
 //
-// The work is 16 values a thread, a whole block, so its maximum needs no exchange.
+// The work is 16 values a thread, a whole block, so its maximum needs no exchange.  Measured, BF16, inputs partly in L2 as a layer's
+// are; in brackets the bytes at the rate of a copy: 16384 x 1600 by rows 12.7 us (10.3); by columns 19.4, 8 of them the maximum
+// (10.3, 18.3 with x read twice); decode by rows 13.1, of 1600 x 16384 10.5 (10.3); 32768 tokens of two 16 x 64 vectors written to the
+// cache 34.5 us (26.5), as many read back 33 (26.5).
 #include <algorithm>
 
 #include "common.cuh"
@@ -54,7 +58,7 @@ __device__ __forceinline__ void part_of_maximum(const MaximaJob &j, uint32_t cta
 }
 
 // ---- by rows ----------------------------------------------------------------------------------------------------------------
-// WPR warps a row; a thread holds kHeld blocks of it, so a row of up to WPR * 32 * kHeld blocks is read once.  A longer one
+// The row's maximum has to be there before its first code: the row waits in registers.  WPR warps a row; a thread holds kHeld blocks of it, so a row of up to WPR * 32 * kHeld blocks is read once.  A longer one
 // (HELD false) is read twice, the second time out of L2 where it fits.  CTAs behind row_ctas take the maximum of another tensor.
 constexpr int kHeld = 4;
 template <int TYPE, int WPR, bool HELD>
@@ -244,6 +248,7 @@ k_fp4_quantize_columns(const __grid_constant__ ColumnsJobs jobs) {
 }
 
 // ---- reading back -----------------------------------------------------------------------------------------------------------
+// A thread a block, as many threads a row as it has blocks (up to a CTA): values leave in 32-byte pieces, side by side.
 template <int TYPE>
 __global__ void __launch_bounds__(256)
 k_fp4_decode(const uint8_t *bytes, uint64_t row_bytes, const uint8_t *scales, uint32_t layout, const float *scale, bool per_row,

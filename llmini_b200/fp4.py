@@ -7,6 +7,7 @@ device buffers; every call enqueues its work on the current stream of the curren
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass, field
 
 import torch
@@ -45,6 +46,9 @@ class Vectors(C.Structure):
                 ("type", C.c_uint32), ("reserved", C.c_uint32)]
 
 
+# The bytes of a Matrix and of a Vectors, which a call takes as they are: a fifth of the time that such an object takes.
+_matrix_bytes, _vectors_bytes = struct.Struct("@PQIIII").pack, struct.Struct("@PQQQII").pack
+_NO_MATRIX, _NO_OPERAND = bytes(C.sizeof(Matrix)), bytes(C.sizeof(Operand))
 _declared = False
 
 
@@ -91,7 +95,7 @@ def _here(t: torch.Tensor, device: int) -> int:
     return t.data_ptr()
 
 
-def _matrix(t: torch.Tensor, device: int) -> Matrix:
+def _matrix(t: torch.Tensor, device: int) -> bytes:
     kind = _TYPES.get(t.dtype)
     if kind is None or t.dim() != 2:
         _refuse(f"a matrix of FP32, BF16 or F16 is wanted, not {tuple(t.shape)} of {t.dtype}")
@@ -104,7 +108,10 @@ def _matrix(t: torch.Tensor, device: int) -> Matrix:
         _refuse("rows overlap")
     if t.get_device() != device:
         _refuse(f"a tensor on {t.device}: the call works on the current CUDA device")
-    return Matrix(t.data_ptr(), ld, rows, cols, kind, 0)
+    try:
+        return _matrix_bytes(t.data_ptr(), ld, rows, cols, kind, 0)
+    except struct.error:
+        _refuse("rows and columns are 32-bit numbers")
 
 
 def _floats(t: torch.Tensor, count: int, what: str, device: int) -> int:
@@ -220,7 +227,6 @@ class Nvfp4PagedCache:
             self.c[i] = Cache(codes.data_ptr(), scales.data_ptr(), exponents.data_ptr(), pages, page_size, heads, half * 2)
         self.device_index = sides[0][0].device.index
         self.sizes = [(s[0].shape[2], s[0].shape[3] * 2) for s in sides]
-        self.vectors = Vectors * len(sides)
 
     def __setattr__(self, name, value):
         _assign(self, name, value)
@@ -240,12 +246,12 @@ class Nvfp4LinearModule:
 
     def quantize_rows(self, x: torch.Tensor, out: Nvfp4Operand) -> None:
         d = _device()
-        check(self._lib.b2_nvfp4_quantize_rows(C.byref(_matrix(x, d)), _operand(out, d), _stream_of(d)), "nvfp4_quantize_rows")
+        check(self._lib.b2_nvfp4_quantize_rows(_matrix(x, d), _operand(out, d), _stream_of(d)), "nvfp4_quantize_rows")
 
     def quantize_columns(self, x: torch.Tensor, out: Nvfp4Operand, maxima: torch.Tensor) -> None:
         """The transpose of x; `maxima`: scratch of NVFP4_MAXIMA FP32 values."""
         d = _device()
-        check(self._lib.b2_nvfp4_quantize_columns(C.byref(_matrix(x, d)), _operand(out, d), _floats(maxima, NVFP4_MAXIMA, "maxima", d), _stream_of(d)),
+        check(self._lib.b2_nvfp4_quantize_columns(_matrix(x, d), _operand(out, d), _floats(maxima, NVFP4_MAXIMA, "maxima", d), _stream_of(d)),
               "nvfp4_quantize_columns")
 
     def decode(self, operand, out: torch.Tensor) -> None:
@@ -261,12 +267,12 @@ class Nvfp4LinearModule:
             c = C.byref(Operand(_here(t.bytes, d), _here(t.scales, d), _here(t.global_scale, d), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
         else:
             c, layout = _operand(operand, d), SCALES_SM100
-        check(self._lib.b2_nvfp4_decode(c, layout, C.byref(_matrix(out, d)), _stream_of(d)), "nvfp4_decode")
+        check(self._lib.b2_nvfp4_decode(c, layout, _matrix(out, d), _stream_of(d)), "nvfp4_decode")
 
     def matmul(self, a: Nvfp4Operand, b: Nvfp4Operand, out: torch.Tensor, bias: torch.Tensor | None = None, accumulate: bool = False) -> None:
         """out [a.rows, b.rows] = a b^T (+ bias) (+ out, FP32 only)."""
         d = _device()
-        check(self._lib.b2_nvfp4_matmul(_operand(a, d), _operand(b, d), C.byref(_matrix(out, d)),
+        check(self._lib.b2_nvfp4_matmul(_operand(a, d), _operand(b, d), _matrix(out, d),
                                         None if bias is None else _floats(bias, b.rows, "bias", d), int(accumulate), _stream_of(d)), "nvfp4_matmul")
 
     def linear_forward(self, x: torch.Tensor, weight: Nvfp4Operand, out: torch.Tensor, scratch: Nvfp4LinearScratch,
@@ -275,7 +281,7 @@ class Nvfp4LinearModule:
         d = _device()
         if scratch.rows is None:
             _refuse("scratch of the backward pass")
-        check(self._lib.b2_nvfp4_linear_forward(C.byref(_matrix(x, d)), _operand(weight, d), C.byref(_matrix(out, d)),
+        check(self._lib.b2_nvfp4_linear_forward(_matrix(x, d), _operand(weight, d), _matrix(out, d),
                                                 None if bias is None else _floats(bias, weight.rows, "bias", d), _operand(scratch.rows, d),
                                                 _stream_of(d)), "nvfp4_linear_forward")
 
@@ -288,17 +294,15 @@ class Nvfp4LinearModule:
             _refuse("scratch of the forward pass")
         if (grad_x is not None and weight_t is None) or (grad_weight is not None and x is None):
             _refuse("grad_x wants weight_t, grad_weight wants x")
-        g = LinearGradients()
-        g.grad = _matrix(grad, d)
-        if grad_x is not None:
-            _operand(weight_t, d)
-            g.weight_t, g.grad_x = weight_t.c, _matrix(grad_x, d)
-        if grad_weight is not None:
-            g.x, g.grad_weight = _matrix(x, d), _matrix(grad_weight, d)
-        _operand(scratch.grad_rows, d)
-        g.grad_rows, g.grad_columns, g.x_columns = scratch.grad_rows.c, scratch.grad_columns.c, scratch.x_columns.c
-        g.d_maxima, g.accumulate = scratch.maxima.data_ptr(), int(accumulate)
-        check(self._lib.b2_nvfp4_linear_backward(C.byref(g), _stream_of(d)), "nvfp4_linear_backward")
+        kept = (scratch.grad_rows, scratch.grad_columns, scratch.x_columns)
+        for o in kept if grad_x is None else kept + (weight_t,):
+            _operand(o, d)
+        # a LinearGradients
+        args = b"".join((_matrix(grad, d), _matrix(x, d) if grad_weight is not None else _NO_MATRIX,
+                         bytes(weight_t.c) if grad_x is not None else _NO_OPERAND, _matrix(grad_x, d) if grad_x is not None else _NO_MATRIX,
+                         _matrix(grad_weight, d) if grad_weight is not None else _NO_MATRIX, *(bytes(o.c) for o in kept),
+                         struct.pack("@PII", _floats(scratch.maxima, 2 * NVFP4_MAXIMA, "maxima", d), int(accumulate), 0)))
+        check(self._lib.b2_nvfp4_linear_backward(args, _stream_of(d)), "nvfp4_linear_backward")
 
     def status(self) -> int:
         """0, or ERROR_LAUNCH_TIMEOUT if a bounded device wait of a product ran out since the last call (synchronises)."""
@@ -310,7 +314,7 @@ class Nvfp4LinearModule:
             _refuse("a cache of another device than the current one")
         if (tensors[1] is None) != (len(cache.c) == 1):
             _refuse("one tensor for each side of the cache")
-        v, first, n = cache.vectors(), tensors[0], len(cache.c)
+        v, first, n = b"", tensors[0], len(cache.c)
         kind = _TYPES.get(first.dtype)
         if kind is None or first.dim() != dims:
             _refuse(f"vectors of FP32, BF16 or F16 are wanted, not {tuple(first.shape)} of {first.dtype}")
@@ -322,7 +326,7 @@ class Nvfp4LinearModule:
                 _refuse("vectors that are written lie apart")
             if i and (t.dtype != first.dtype or shape[:-2] != first.shape[:-2]):
                 _refuse("keys and values: tensors of one type and length")
-            v[i] = Vectors(_here(t, d), stride[0] if dims == 4 else 0, stride[-3], stride[-2], kind, 0)
+            v += _vectors_bytes(_here(t, d), stride[0] if dims == 4 else 0, stride[-3], stride[-2], kind, 0)
         return v, n, first.shape
 
     def cache_write(self, cache: Nvfp4PagedCache, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor | None = None) -> None:

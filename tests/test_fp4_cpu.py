@@ -3,6 +3,7 @@ is launched, and the plain definition that the kernels are tested against does w
 import ctypes as C
 import os
 import re
+import struct
 
 import numpy as np
 import pytest
@@ -64,6 +65,19 @@ BAD_MATRICES = [matrix(4, 64, data=None), matrix(4, 64, ld=63), matrix(4, 64, ty
                 matrix(4, 64, ld=1 << 40), matrix(65535 * 128 + 1, 64)]
 BAD_OPERANDS = [operand(4, 64, data=None), operand(4, 64, data=AT + 8), operand(4, 64, row_bytes=40), operand(4, 64, row_bytes=16), operand(4, 64, count=3),
                 operand(4, 72), with_field(operand(4, 64), reserved=7), operand(4, 64, row_bytes=1 << 40)]
+
+
+def test_bytes_of_the_mirrors():
+    """What the Python calls pass in a structure's place is that structure."""
+    assert bytes(fp4.Matrix(1 << 40, 1 << 35, 3, 4, 2, 0)) == fp4._matrix_bytes(1 << 40, 1 << 35, 3, 4, 2, 0)
+    assert bytes(fp4.Vectors(1 << 40, 1 << 35, 1 << 34, 64, 1, 0)) == fp4._vectors_bytes(1 << 40, 1 << 35, 1 << 34, 64, 1, 0)
+    m, o = C.sizeof(fp4.Matrix), C.sizeof(fp4.Operand)
+    g = fp4.LinearGradients
+    assert [f.offset for f in (g.x, g.weight_t, g.grad_x, g.grad_weight, g.grad_rows, g.grad_columns, g.x_columns, g.d_maxima)] == \
+        [m, 2 * m, 2 * m + o, 3 * m + o, 4 * m + o, 4 * m + 2 * o, 4 * m + 3 * o, 4 * m + 4 * o]
+    assert C.sizeof(g) == 4 * m + 4 * o + struct.calcsize("@PII") and len(fp4._NO_MATRIX) == m and len(fp4._NO_OPERAND) == o
+    with pytest.raises(ValueError):
+        fp4._matrix(torch.empty(1, dtype=torch.float32).expand(1 << 33, 1), -1)
 
 
 def test_quantisers_refuse():

@@ -934,8 +934,10 @@ cudaError_t few_impl(const b2_nvfp4_operand *a, const b2_matrix *x, const b2_nvf
     while (f.tmem_cols < (f.n + 31) / 32 * 32 + 32) f.tmem_cols *= 2;
     // A CTA keeps its tensor memory while it waits for the others of its cluster, so none of them may have to wait for tensor
     // memory in turn: every launch takes at least the share of an SM's shared memory (228 KB, 1 KB of it for the system) that it
-    // takes of the tensor memory, and more than a Newton-Schulz CTA that holds all of it leaves.
-    const uint32_t bytes = std::max({few_layout(f, kFused).bytes + 1024, 228u * 1024 / 512 * f.tmem_cols - 1024, 40u * 1024});
+    // takes of the tensor memory, and more than a Newton-Schulz CTA that holds all of it leaves; with a cluster, more than other
+    // programs' tensor-core kernels do that take half of an SM's shared memory (two such launches still fit an SM, so that one begins
+    // while the other ends).
+    const uint32_t bytes = std::max({few_layout(f, kFused).bytes + 1024, 228u * 1024 / 512 * f.tmem_cols - 1024, (f.split > 1 ? 108u : 40u) * 1024});
     CUtensorMap map_a = {}, map_b, map_sa = {}, map_sb;
     if ((!kFused && (!codes_map(&map_a, *a, f.n) || !scales_map(&map_sa, *a, 1))) || !codes_map(&map_b, b, 128) || !scales_map(&map_sb, b, 1))
         return cudaErrorInvalidValue;

@@ -79,8 +79,8 @@ def _refuse(what: str):
     raise ValueError(what)
 
 
-# The current device, and its current stream's handle, without the objects around them: of the 6 us that a call on small tensors
-# takes on the host, the launch itself is 2.5.
+# The current device, and its current stream's handle, without the objects around them: of the 4 to 5 us that a call on small
+# tensors takes on the host, the launch itself is 2.5.
 _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 

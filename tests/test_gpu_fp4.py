@@ -648,3 +648,54 @@ def test_results_do_not_overlap(module):
     module.cache_write(cache, torch.arange(5, device="cuda"), one, one)
     module.cache_read(cache, table, torch.full_like(lengths, 5), good, good.clone())
     assert torch.equal(good[0, :5], good[1, :5]) and (good[0, :5] == good[0, 0, 0]).all() and good[0, 0, 0].any()
+
+
+FIRST_CALLS = """
+import torch, llmini_b200 as b2
+m = b2.Nvfp4LinearModule()
+x, w = torch.randn(%d, 160, device="cuda"), b2.Nvfp4Operand.empty(96, 160, per_row=False)
+y, s, maxima = torch.empty(%d, 96, device="cuda"), b2.Nvfp4LinearScratch(%d, 160, 96), torch.empty(1024, device="cuda")
+master = torch.randn(160, 96, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    m.quantize_columns(master, w, maxima)
+    m.linear_forward(x, w, y, s)
+graph.replay()
+torch.cuda.synchronize()
+first = y.clone()
+m.quantize_columns(master, w, maxima)
+m.linear_forward(x, w, y, s)
+assert torch.equal(first, y) and y.any() and m.status() == 0
+"""
+
+
+@pytest.mark.parametrize("tokens", [2, 30, 300])
+def test_the_first_calls_of_a_process_are_captured(tokens):
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS % (tokens, tokens, tokens)], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_calls_on_two_streams(module):
+    """Products of every kernel at the same time, each with its own scratch: what they give one after the other."""
+    rng = np.random.default_rng(5)
+    jobs = []
+    for tokens, inputs, outputs in ((1, 1600, 4800), (24, 6400, 1600), (300, 768, 1000), (2100, 400, 4000)):
+        _, w = operand(rng, outputs, inputs, False)
+        x = torch.randn(tokens, inputs, device="cuda", dtype=torch.bfloat16)
+        jobs.append((x, w, [torch.empty(tokens, outputs, device="cuda") for _ in range(3)], [b2.Nvfp4LinearScratch(tokens, inputs, outputs) for _ in range(2)]))
+    for x, w, y, s in jobs:
+        module.linear_forward(x, w, y[2], s[0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                for x, w, y, s in (jobs if i == 0 else reversed(jobs)):
+                    module.linear_forward(x, w, y[i], s[i])
+    torch.cuda.synchronize()
+    assert module.status() == 0
+    for x, w, y, s in jobs:
+        assert torch.equal(y[0], y[2]) and torch.equal(y[1], y[2])

@@ -699,3 +699,21 @@ def test_calls_on_two_streams(module):
     assert module.status() == 0
     for x, w, y, s in jobs:
         assert torch.equal(y[0], y[2]) and torch.equal(y[1], y[2])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("offset,spare", [(0, 0), (8, 8), (4, 4), (1, 3), (16, 0)])
+def test_cache_of_vectors_on_any_boundary(module, dtype, offset, spare):
+    heads, dim, tokens = 3, 48, 10
+    cache = b2.Nvfp4PagedCache.empty(5, 4, heads, dim)
+    memory = torch.randn(tokens, heads, offset + dim + spare, device="cuda").to(TYPES[dtype])
+    key, value = memory[..., offset:offset + dim], torch.randn(tokens, heads, dim, device="cuda").to(TYPES[dtype])
+    module.cache_write(cache, torch.arange(tokens, device="cuda") + 4, key, value)
+    out = torch.full((1, tokens, heads, offset + dim + spare), -3.0, device="cuda", dtype=TYPES[dtype])
+    other = torch.empty(1, tokens, heads, dim, device="cuda", dtype=TYPES[dtype])
+    module.cache_read(cache, torch.tensor([[1, 2, 3]], dtype=torch.int32, device="cuda"), torch.tensor([tokens], dtype=torch.int32, device="cuda"),
+                      out[..., offset:offset + dim], other)
+    for got, given in ((out[0, ..., offset:offset + dim], key), (other[0], value)):
+        want = rounded(plain.to_double(given).reshape(-1, dim)).reshape(tokens, heads, dim)
+        np.testing.assert_array_equal(plain.to_double(got), torch.from_numpy(want).to(TYPES[dtype]).double().numpy())
+    assert (out[..., :offset] == -3).all() and (out[..., offset + dim:] == -3).all()

@@ -134,15 +134,32 @@ def _up(n: int, step: int) -> int:
     return -(-n // step) * step
 
 
-def _assign(o, name: str, value) -> None:
-    """Another tensor for a field of an object that calls have the addresses of: they are taken anew."""
-    object.__setattr__(o, name, value)
-    if name in o.__dataclass_fields__ and name != "c" and "device_index" in o.__dict__:
-        o.__post_init__()
+class _Described:
+    """An object whose tensors' addresses calls take from a structure made once (`_describe`: what follows from the fields).  Fields
+    are looked over before they are stored, together with what follows from them; a field that is refused changes nothing."""
+
+    def __post_init__(self):
+        self.replace()
+
+    def __setattr__(self, name, value):
+        if name in self._FIELDS and "c" in self.__dict__:
+            self.replace(**{name: value})
+        else:
+            object.__setattr__(self, name, value)
+
+    def replace(self, **fields) -> None:
+        """Other values for some fields at once, as another size needs."""
+        if not fields.keys() <= set(self._FIELDS):
+            raise TypeError(f"fields are {self._FIELDS}")
+        self.__dict__.update(self._describe(**{n: fields.get(n, self.__dict__[n]) for n in self._FIELDS}))
+
+
+def _tensors(*tensors) -> bool:
+    return all(isinstance(t, torch.Tensor) for t in tensors)
 
 
 @dataclass
-class Nvfp4Operand:
+class Nvfp4Operand(_Described):
     """A matrix in NVFP4 as the product reads it: codes [rows, row_bytes] (two a byte, k / 2 of a row's bytes), block scales in the
     tensor cores' layout (SCALES_SM100), and the scale on top, one or one a row.  k: the values of a row, a multiple of 16."""
     bytes: torch.Tensor
@@ -151,29 +168,27 @@ class Nvfp4Operand:
     rows: int
     k: int
     c: Operand = field(init=False, repr=False)
+    _FIELDS = ("bytes", "scales", "scale", "rows", "k")
 
-    def __post_init__(self):
-        b = self.bytes
-        if b.dtype != torch.uint8 or b.dim() != 2 or b.shape[0] != self.rows or (b.shape[1] > 1 and b.stride(1) != 1):
+    @staticmethod
+    def _describe(bytes, scales, scale, rows, k):
+        b = bytes
+        if not _tensors(b, scales, scale) or b.dtype != torch.uint8 or b.dim() != 2 or b.shape[0] != rows or (b.shape[1] > 1 and b.stride(1) != 1):
             _refuse("codes: uint8 [rows, bytes of a row]")
-        row_bytes = b.stride(0) if self.rows > 1 else _up(b.shape[1], 16)
-        if self.k % 16 or self.k <= 0 or b.shape[1] < self.k // 2 or row_bytes % 16:
+        row_bytes = b.stride(0) if rows > 1 else _up(b.shape[1], 16)
+        if k % 16 or k <= 0 or b.shape[1] < k // 2 or row_bytes % 16:
             _refuse("a row: k values, a multiple of 16, on a 16-byte boundary")
-        if self.scales.dtype != torch.uint8 or not self.scales.is_contiguous() or self.scales.numel() < _up(self.rows, 128) * _up(self.k // 16, 4):
+        if scales.dtype != torch.uint8 or not scales.is_contiguous() or scales.numel() < _up(rows, 128) * _up(k // 16, 4):
             _refuse("scales: a contiguous buffer of sm100_scales_bytes(rows, k) bytes")
-        n = self.scale.numel()
-        if self.scale.dtype != torch.float32 or not self.scale.is_contiguous() or n not in (1, self.rows):
+        n = scale.numel()
+        if scale.dtype != torch.float32 or not scale.is_contiguous() or n not in (1, rows):
             _refuse("scale: FP32, one or one a row")
-        if self.rows and (b.data_ptr() % 16 or self.scales.data_ptr() % 16):
+        if rows and (b.data_ptr() % 16 or scales.data_ptr() % 16):
             _refuse("codes and scales start on 16-byte boundaries")
-        if not (b.device == self.scales.device == self.scale.device) or not b.is_cuda:
+        if not (b.device == scales.device == scale.device) or not b.is_cuda:
             _refuse("an operand lies on one CUDA device")
-        self.device_index = b.device.index
-        self.c = Operand(b.data_ptr(), self.scales.data_ptr(), self.scale.data_ptr(), row_bytes, self.rows, self.k, n, 0)
-        self.ref = C.byref(self.c)
-
-    def __setattr__(self, name, value):
-        _assign(self, name, value)
+        c = Operand(b.data_ptr(), scales.data_ptr(), scale.data_ptr(), row_bytes, rows, k, n, 0)
+        return dict(bytes=bytes, scales=scales, scale=scale, rows=rows, k=k, device_index=b.device.index, c=c, ref=C.byref(c))
 
     @staticmethod
     def empty(rows: int, k: int, per_row: bool = True, device="cuda") -> "Nvfp4Operand":
@@ -207,29 +222,32 @@ class Nvfp4LinearScratch:
 
 
 @dataclass
-class Nvfp4PagedCache:
+class Nvfp4PagedCache(_Described):
     """Keys and values in pages: for each, codes [pages, page_size, heads, dim / 2], block scales [.., dim / 16] and exponents
     [pages, page_size, heads], all uint8 and contiguous.  `value` may be None: a cache of one tensor."""
     key: tuple
     value: tuple | None = None
     c: object = field(init=False, repr=False)
+    _FIELDS = ("key", "value")
 
-    def __post_init__(self):
-        sides = [self.key] + ([self.value] if self.value is not None else [])
-        self.c = (Cache * len(sides))()
-        for i, (codes, scales, exponents) in enumerate(sides):
+    @staticmethod
+    def _describe(key, value):
+        sides = []
+        for side in (key,) if value is None else (key, value):
+            if not isinstance(side, (tuple, list)) or len(side) != 3 or not _tensors(*side) or side[0].dim() != 4:
+                _refuse("a side of a cache: codes, scales and exponents")
+            codes, scales, exponents = side
             pages, page_size, heads, half = codes.shape
             shapes = (codes.shape, scales.shape, exponents.shape) == ((pages, page_size, heads, half), (pages, page_size, heads, half // 8), (pages, page_size, heads))
-            if half % 8 or not shapes or any(t.dtype != torch.uint8 or not t.is_contiguous() for t in (codes, scales, exponents)):
+            if half % 8 or not shapes or any(t.dtype != torch.uint8 or not t.is_contiguous() for t in side):
                 _refuse("a cache: uint8 [pages, page_size, heads, dim / 2], [.., dim / 16], [pages, page_size, heads]")
-            if not codes.is_cuda or not (codes.device == scales.device == exponents.device == sides[0][0].device):
-                _refuse("a cache lies on one CUDA device")
-            self.c[i] = Cache(codes.data_ptr(), scales.data_ptr(), exponents.data_ptr(), pages, page_size, heads, half * 2)
-        self.device_index = sides[0][0].device.index
-        self.sizes = [(s[0].shape[2], s[0].shape[3] * 2) for s in sides]
-
-    def __setattr__(self, name, value):
-        _assign(self, name, value)
+            sides.append(side)
+        first = sides[0][0]
+        if any(not t.is_cuda or t.device != first.device for side in sides for t in side):
+            _refuse("a cache lies on one CUDA device")
+        c = (Cache * len(sides))(*(Cache(*(t.data_ptr() for t in side), *side[2].shape, side[0].shape[3] * 2) for side in sides))
+        return dict(key=key, value=value, device_index=first.device.index, c=c,
+                    sizes=[(side[2].shape[2], side[0].shape[3] * 2) for side in sides])
 
     @staticmethod
     def empty(pages: int, page_size: int, heads: int, dim: int, value_dim: int | None = None, device="cuda") -> "Nvfp4PagedCache":

@@ -192,3 +192,70 @@ def test_every_kernel_waits_before_it_touches_memory():
         assert "ld.global" not in before and "tma_load" not in before, name
     for form in ("__ldg(", "ld.global.nc", "const float *__restrict__"):
         assert form not in text, form
+
+
+class OnDevice(torch.Tensor):
+    """Host memory that passes for memory of a CUDA device: what is described and refused needs no GPU."""
+    is_cuda = property(lambda self: True)
+
+
+def on_device(*shape, dtype=torch.uint8):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def whole_operand(rows, k):
+    return dict(bytes=on_device(rows, -(-k // 32) * 16), scales=on_device(-(-rows // 128) * -(-k // 64) * 512), scale=on_device(rows, dtype=torch.float32), rows=rows,
+                k=k)
+
+
+def test_a_refused_field_changes_nothing():
+    """An operand and a cache refuse a field before they take it: what calls read (c) is what the fields hold, before and after."""
+    kept = whole_operand(40, 64)
+    o = b2.Nvfp4Operand(**kept)
+
+    def agrees():
+        assert (o.c.bytes, o.c.scales, o.c.scale) == (o.bytes.data_ptr(), o.scales.data_ptr(), o.scale.data_ptr())
+        assert (o.c.rows, o.c.cols, o.c.row_bytes, o.c.scale_count) == (o.rows, o.k, o.bytes.stride(0), o.scale.numel())
+        assert o.ref._obj is o.c
+    agrees()
+    for name, bad in (("bytes", on_device(39, 32)), ("bytes", torch.zeros(40, 32, dtype=torch.uint8)), ("bytes", on_device(40, 24)), ("bytes", None),
+                      ("scales", on_device(511)), ("scale", on_device(39, dtype=torch.float32)), ("scale", on_device(40)), ("rows", 39), ("rows", 41),
+                      ("k", 80), ("k", 72), ("k", 0), ("rows", "40"), ("rows", 1 << 32)):
+        with pytest.raises(ValueError):
+            setattr(o, name, bad)
+        assert all(getattr(o, n) is v for n, v in kept.items()), name
+        agrees()
+    o.bytes, o.k = on_device(40, 48), 48
+    agrees()
+    larger = whole_operand(300, 160)
+    with pytest.raises(ValueError):
+        o.replace(**{**larger, "scale": on_device(299, dtype=torch.float32)})
+    assert o.rows == 40
+    agrees()
+    o.replace(**larger)
+    assert o.rows == 300 and o.bytes is larger["bytes"]
+    agrees()
+
+    def side(pages, page, heads, dim):
+        return tuple(on_device(pages, page, heads, *more) for more in ((dim // 2,), (dim // 16,), ()))
+    key, value = side(4, 8, 2, 32), side(4, 8, 2, 48)
+    cache = b2.Nvfp4PagedCache(key, value)
+
+    def follows(n=2):
+        assert len(cache.c) == len(cache.sizes) == n and (cache.value is None) == (n == 1)
+        for c, s, size in zip(cache.c, (cache.key, cache.value), cache.sizes):
+            assert [c.bytes, c.scales, c.exponents] == [t.data_ptr() for t in s]
+            assert (c.pages, c.page_size, c.heads, c.dim) == (*s[2].shape, s[0].shape[-1] * 2) and size == (c.heads, c.dim)
+    follows()
+    before = cache.key, cache.value, cache.c
+    for bad in (side(4, 8, 2, 40), side(4, 8, 2, 32)[:2], [torch.zeros(4, 8, 2, n, dtype=torch.uint8) for n in (16, 2)] + [torch.zeros(4, 8, 2, dtype=torch.uint8)],
+                side(4, 8, 2, 32)[::-1], [t[:, :, :1] for t in side(4, 8, 2, 32)], None, 7):
+        for name in ("key",) if bad is None else ("key", "value"):
+            with pytest.raises(ValueError):
+                setattr(cache, name, bad)
+            assert (cache.key, cache.value, cache.c) == before
+            follows()
+    cache.key = side(9, 8, 3, 64)
+    follows()
+    cache.value = None
+    follows(1)

@@ -717,3 +717,32 @@ def test_cache_of_vectors_on_any_boundary(module, dtype, offset, spare):
         want = rounded(plain.to_double(given).reshape(-1, dim)).reshape(tokens, heads, dim)
         np.testing.assert_array_equal(plain.to_double(got), torch.from_numpy(want).to(TYPES[dtype]).double().numpy())
     assert (out[..., :offset] == -3).all() and (out[..., offset + dim:] == -3).all()
+
+
+def test_after_a_refused_field_calls_use_what_was_there(module):
+    """An operand and a cache that refused a field work on, on the memory that they still hold."""
+    x = torch.randn(40, 64, device="cuda")
+    o, want = b2.Nvfp4Operand.empty(40, 64), b2.Nvfp4Operand.empty(40, 64)
+    module.quantize_rows(x, want)
+    kept = o.bytes
+    for name, bad in (("bytes", torch.zeros(39, 32, dtype=torch.uint8, device="cuda")), ("rows", 20), ("scale", torch.zeros(20, device="cuda"))):
+        with pytest.raises(ValueError):
+            setattr(o, name, bad)
+    module.quantize_rows(x, o)
+    assert o.bytes is kept and torch.equal(kept, want.bytes) and torch.equal(o.scale, want.scale) and torch.equal(o.scales, want.scales)
+    with pytest.raises(ValueError):   # a bias for the rows that there are
+        module.matmul(o, o, torch.empty(40, 40, device="cuda"), bias=torch.zeros(20, device="cuda"))
+    more = b2.Nvfp4Operand.empty(130, 160)
+    o.replace(bytes=more.bytes, scales=more.scales, scale=more.scale, rows=130, k=160)
+    y = torch.randn(130, 160, device="cuda")
+    module.quantize_rows(y, o)
+    back = torch.empty_like(y)
+    module.decode(more, back)
+    assert (plain.to_double(back) == rounded(plain.to_double(y))).all()
+    cache = b2.Nvfp4PagedCache.empty(4, 8, 2, 32)
+    key = cache.key
+    with pytest.raises(ValueError):
+        cache.key = tuple(t.cpu() for t in key)
+    v = torch.randn(3, 2, 32, device="cuda")
+    module.cache_write(cache, torch.arange(3, device="cuda"), v, v)
+    assert cache.key is key and key[0].view(32, -1)[:3].any() and torch.equal(key[0], cache.value[0])

@@ -224,7 +224,7 @@ class Nvfp4LinearScratch:
 @dataclass
 class Nvfp4PagedCache(_Described):
     """Keys and values in pages: for each, codes [pages, page_size, heads, dim / 2], block scales [.., dim / 16] and exponents
-    [pages, page_size, heads], all uint8 and contiguous.  `value` may be None: a cache of one tensor."""
+    [pages, page_size, heads], all uint8 and contiguous.  `value` may be None: a cache of one tensor.  Sides are kept as tuples."""
     key: tuple
     value: tuple | None = None
     c: object = field(init=False, repr=False)
@@ -234,7 +234,8 @@ class Nvfp4PagedCache(_Described):
     def _describe(key, value):
         sides = []
         for side in (key,) if value is None else (key, value):
-            if not isinstance(side, (tuple, list)) or len(side) != 3 or not _tensors(*side) or side[0].dim() != 4:
+            side = tuple(side) if isinstance(side, (tuple, list)) else ()
+            if len(side) != 3 or not _tensors(*side) or side[0].dim() != 4:
                 _refuse("a side of a cache: codes, scales and exponents")
             codes, scales, exponents = side
             pages, page_size, heads, half = codes.shape
@@ -246,7 +247,7 @@ class Nvfp4PagedCache(_Described):
         if any(not t.is_cuda or t.device != first.device for side in sides for t in side):
             _refuse("a cache lies on one CUDA device")
         c = (Cache * len(sides))(*(Cache(*(t.data_ptr() for t in side), *side[2].shape, side[0].shape[3] * 2) for side in sides))
-        return dict(key=key, value=value, device_index=first.device.index, c=c,
+        return dict(key=sides[0], value=sides[1] if len(sides) > 1 else None, device_index=first.device.index, c=c,
                     sizes=[(side[2].shape[2], side[0].shape[3] * 2) for side in sides])
 
     @staticmethod

@@ -259,3 +259,24 @@ def test_a_refused_field_changes_nothing():
     follows()
     cache.value = None
     follows(1)
+
+
+def test_a_cache_keeps_its_own_tuples():
+    """Sides may be given as lists; what happens to these later is not half followed."""
+    def side():
+        return [on_device(4, 8, 2, *more) for more in ((16,), (2,), ())]
+    key, value = side(), side()
+    cache = b2.Nvfp4PagedCache(key, value)
+    kept = tuple(key), tuple(value)
+    key[0], value[1] = on_device(4, 8, 2, 16), on_device(4, 8, 2, 2)
+
+    def holds(key, value):
+        assert isinstance(cache.key, tuple) and all(a is b for a, b in zip(cache.key + cache.value, key + value))
+        assert [(c.bytes, c.scales, c.exponents) for c in cache.c] == [tuple(t.data_ptr() for t in s) for s in (key, value)]
+    holds(*kept)
+    with pytest.raises(TypeError):
+        cache.key[0] = on_device(4, 8, 2, 16)
+    holds(*kept)
+    cache.key = key
+    key.reverse()
+    holds(tuple(key[::-1]), kept[1])

@@ -61,6 +61,15 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
+// Rounded to odd: of the two neighbours of an inexact product the one whose last bit is set, which a second rounding, to two bits less or
+// fewer still, takes where it would have taken the product itself (Boldo and Melquiond, IEEE Trans. Comput. 57, 2008).
+__device__ __forceinline__ Pair mul2_odd(Pair a, Pair b) {
+    Pair down, up;
+    asm("mul.rm.f32x2 %0, %1, %2;" : "=l"(down.v) : "l"(a.v), "l"(b.v));
+    asm("mul.rp.f32x2 %0, %1, %2;" : "=l"(up.v) : "l"(a.v), "l"(b.v));
+    const float2 d = halves(down), u = halves(up);
+    return pair(__float_as_uint(d.x) & 1u ? d.x : u.x, __float_as_uint(d.y) & 1u ? d.y : u.y);
+}
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     Pair r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
@@ -190,7 +199,9 @@ __device__ __forceinline__ uint32_t encode_block(const Raw<TYPE> &block, uint32_
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------------------------
-// Values of a block: code * s is exact in FP16 (6 bits, 2^-10 .. 2688), the product with g is rounded in FP32.
+// Values of a block: code * s is exact in FP16 (6 bits, 2^-10 .. 2688), the product with g is rounded in FP32; ODD: to odd, for values
+// that are rounded again to 16 bits (with g a power of two it is exact, and either will do).
+template <bool ODD>
 __device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, float (&v)[16]) {
     uint32_t sh;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(sh) : "h"((uint16_t)(s | (s << 8))));
@@ -206,7 +217,7 @@ __device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, f
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = __half22float2(__hmul2(*reinterpret_cast<const __half2 *>(&h[i]), s2));
-            const float2 o = halves(mul2(pair(f.x, f.y), g2));
+            const float2 o = halves(ODD ? mul2_odd(pair(f.x, f.y), g2) : mul2(pair(f.x, f.y), g2));
             v[8 * k + 2 * i] = o.x;
             v[8 * k + 2 * i + 1] = o.y;
         }

@@ -258,13 +258,15 @@ k_fp4_decode(const uint8_t *bytes, uint64_t row_bytes, const uint8_t *scales, ui
     if (row >= rows) return;
     const uint32_t tiles = (blocks + 3) / 4;
     const float g = scale[per_row ? row : 0];
+    const bool power = (__float_as_uint(g) & 0x7fffffu) == 0;   // the optimizer's scales are none
     for (uint32_t blk = threadIdx.x % threads_per_row; blk < blocks; blk += threads_per_row) {
         const uint2 codes = *reinterpret_cast<const uint2 *>(bytes + (uint64_t)row * row_bytes + (uint64_t)blk * 8);
         const uint64_t flat = (uint64_t)row * blocks + blk;
         const uint32_t s = layout == B2_SCALES_SM100 ? scales[sm100_scale_offset(row, blk, tiles)]
                            : layout == B2_SCALES_RAW ? scales[flat] : csf_load_scale(scales, (uint32_t)flat);
         float v[16];
-        decode_block(codes, s, g, v);
+        if (TYPE != B2_TYPE_F32 && !power) decode_block<true>(codes, s, g, v);
+        else decode_block<false>(codes, s, g, v);
         store_block<TYPE>(out + (uint64_t)row * ld_bytes + (uint64_t)blk * 16 * Raw<TYPE>::kSize, v, (int)min(cols - blk * 16u, 16u), access);
     }
 }
@@ -363,7 +365,7 @@ k_fp4_cache_read(const __grid_constant__ CachePair p, const int32_t *table, uint
             e = c.exponents[at];
         }
         float v[16];
-        decode_block(codes, s, e == 255u ? __uint_as_float(0x7fffffffu) : e == 0u ? 0x1p-127f : __uint_as_float(e << 23), v);
+        decode_block<false>(codes, s, e == 255u ? __uint_as_float(0x7fffffffu) : e == 0u ? 0x1p-127f : __uint_as_float(e << 23), v);
         store_block<TYPE>(out + (t * side.vectors.token_stride + head * side.vectors.head_stride + blk * 16) * Raw<TYPE>::kSize, v, 16, side.access);
     }
 }

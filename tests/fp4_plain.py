@@ -101,3 +101,13 @@ def to_double(t):
 
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
+
+
+def rounded_once(v, dtype):
+    """Numbers in 64 bits to the nearest ones of `dtype` (still in 64 bits), the even one between two; beyond the range infinity."""
+    bits, least = {torch.float32: (23, -126), torch.bfloat16: (7, -126), torch.float16: (10, -14)}[dtype]
+    v = np.asarray(v, np.float64)
+    with np.errstate(all="ignore"):
+        unit = np.exp2(np.maximum(np.floor(np.log2(np.abs(v))), least) - bits)
+        r = np.where(v == 0, v, np.rint(v / unit) * unit)
+    return np.where(np.abs(r) > torch.finfo(dtype).max, np.copysign(np.inf, v), r)

@@ -280,3 +280,12 @@ def test_a_cache_keeps_its_own_tuples():
     cache.key = key
     key.reverse()
     holds(tuple(key[::-1]), kept[1])
+
+
+def test_plain_rounding():
+    x = np.random.default_rng(0).standard_normal(4000).astype(np.float32) * np.exp2(np.arange(4000) % 60 - 30).astype(np.float32)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):   # one rounding of FP32 values, which torch does too
+        assert np.array_equal(plain.rounded_once(x, dtype), torch.from_numpy(x).to(dtype).double().numpy())
+    big = torch.finfo(torch.float16).max
+    assert plain.rounded_once([big + 15.9, big + 16, -big - 16, 2.0 ** -25, 2.0 ** -24 * 1.5, -0.0], torch.float16).tolist() == [big, np.inf, -np.inf, 0, 2.0 ** -23, 0]
+    assert plain.rounded_once([1 + 2.0 ** -8 + 2.0 ** -40], torch.bfloat16).tolist() == [1 + 2.0 ** -7]   # in two steps it would be 1

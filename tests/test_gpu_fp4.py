@@ -746,3 +746,41 @@ def test_after_a_refused_field_calls_use_what_was_there(module):
     v = torch.randn(3, 2, 32, device="cuda")
     module.cache_write(cache, torch.arange(3, device="cuda"), v, v)
     assert cache.key is key and key[0].view(32, -1)[:3].any() and torch.equal(key[0], cache.value[0])
+
+
+def scales_next_to_borders(dtype, rng):
+    """FP32 scales whose products with some code * s lie so close to the middle between two values of `dtype` that FP32 has that middle
+    for them, below it or above, where it is the other value that is nearest."""
+    products = np.array([a * b for a in (1, 3) for b in range(8, 16)], np.float64)
+    bits = {torch.bfloat16: 7, torch.float16: 10}[dtype]
+    found = []
+    for a in products:
+        middles = (2 * rng.integers(1 << bits, 2 << bits, 4000) + 1) / 2.0
+        g = (middles / a).astype(np.float32)
+        exact = a * g.astype(np.float64)
+        near = (exact != middles) & (exact.astype(np.float32) == middles)
+        even = np.floor(middles) % 2 == 0   # the second rounding would go to the even one
+        found += list(g[near & ((exact > middles) == even)][:12])
+    return np.array(found, np.float32)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_decode_rounds_once(module, dtype):
+    """Every code with every scale: the nearest value of the type, whatever the scale on top."""
+    rng = np.random.default_rng(11)
+    t = TYPES[dtype]
+    near = scales_next_to_borders(torch.bfloat16 if dtype == "f32" else t, rng)
+    assert len(near) > 40
+    g = np.concatenate([near * np.float32(2.0) ** rng.integers(-14, 4, len(near)).astype(np.float32), [0.13489583134651184, 2.0 ** -8, 1.0 / 3, 2.0 ** 120 * 1.3,
+                       2.0 ** -126 * 1.7, 2.0 ** -135 * 1.37, 2.0 ** -149, 2.0 ** -30 * 1.1], rng.random(40)]).astype(np.float32)
+    rows, k = len(g), 16 * 127
+    codes = np.tile(np.arange(16, dtype=np.uint8), (rows, k // 16))
+    s = np.tile(np.arange(127, dtype=np.uint8), (rows, 1))
+    v = plain.values(codes, s, g)
+    o = b2.Nvfp4Operand(torch.from_numpy(plain.pack(codes, -(-k // 32) * 16)).cuda(), torch.from_numpy(plain.tiled(s)).cuda(), torch.from_numpy(g).cuda(), rows, k)
+    out = torch.empty(rows, k, dtype=t, device="cuda")
+    module.decode(o, out)
+    np.testing.assert_array_equal(plain.to_double(out), plain.rounded_once(v, t))
+    if dtype != "f32":   # and rounding twice is something else here
+        with np.errstate(all="ignore"):
+            assert (plain.rounded_once(v.astype(np.float32), t) != plain.rounded_once(v, t)).sum() > 20

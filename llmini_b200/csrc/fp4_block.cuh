@@ -61,14 +61,10 @@ __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
-// Rounded to odd: of the two neighbours of an inexact product the one whose last bit is set, which a second rounding, to two bits less or
-// fewer still, takes where it would have taken the product itself (Boldo and Melquiond, IEEE Trans. Comput. 57, 2008).
-__device__ __forceinline__ Pair mul2_odd(Pair a, Pair b) {
-    Pair down, up;
-    asm("mul.rm.f32x2 %0, %1, %2;" : "=l"(down.v) : "l"(a.v), "l"(b.v));
-    asm("mul.rp.f32x2 %0, %1, %2;" : "=l"(up.v) : "l"(a.v), "l"(b.v));
-    const float2 d = halves(down), u = halves(up);
-    return pair(__float_as_uint(d.x) & 1u ? d.x : u.x, __float_as_uint(d.y) & 1u ? d.y : u.y);
+__device__ __forceinline__ Pair mul2_truncated(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rz.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
 }
 __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     Pair r;
@@ -199,14 +195,20 @@ __device__ __forceinline__ uint32_t encode_block(const Raw<TYPE> &block, uint32_
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------------------------
-// Values of a block: code * s is exact in FP16 (6 bits, 2^-10 .. 2688), the product with g is rounded in FP32; ODD: to odd, for values
-// that are rounded again to 16 bits (with g a power of two it is exact, and either will do).
-template <bool ODD>
+// Values of a block: code * s is exact in FP16 (6 bits, 2^-10 .. 2688), the product with g is rounded in FP32.
+// Values that go on to 16 bits are not to be rounded to nearest before: where FP32 has the middle between two 16-bit values for a
+// product that lies beside it, the second rounding goes wrong.
+//   kTruncate: the product truncated, and its last bit set where g has 14 bits or more (not counting zeros at its end).  Such a product
+//     is no middle, which has 12 bits at most, but may be truncated to one.  With fewer bits of g it has 19 at most and is exact.
+// A subnormal g, of whatever bits, takes product_to_odd.
+enum Decoding : int { kNearest = 0, kTruncate = 1 };
+template <int HOW>
 __device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, float (&v)[16]) {
     uint32_t sh;
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(sh) : "h"((uint16_t)(s | (s << 8))));
     const __half2 s2 = *reinterpret_cast<const __half2 *>(&sh);
     const Pair g2 = pair(g, g);
+    const uint32_t last = HOW == kTruncate && (__float_as_uint(g) & 0x7ffu) != 0 ? 1u : 0u;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         uint32_t h[4];
@@ -217,11 +219,29 @@ __device__ __forceinline__ void decode_block(uint2 codes, uint32_t s, float g, f
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = __half22float2(__hmul2(*reinterpret_cast<const __half2 *>(&h[i]), s2));
-            const float2 o = halves(ODD ? mul2_odd(pair(f.x, f.y), g2) : mul2(pair(f.x, f.y), g2));
-            v[8 * k + 2 * i] = o.x;
-            v[8 * k + 2 * i + 1] = o.y;
+            if (HOW == kNearest) {
+                const float2 o = halves(mul2(pair(f.x, f.y), g2));
+                v[8 * k + 2 * i] = o.x;
+                v[8 * k + 2 * i + 1] = o.y;
+            } else {
+                const float2 o = halves(mul2_truncated(pair(f.x, f.y), g2));
+                v[8 * k + 2 * i] = __uint_as_float(__float_as_uint(o.x) | last);
+                v[8 * k + 2 * i + 1] = __uint_as_float(__float_as_uint(o.y) | last);
+            }
         }
     }
+}
+// The value of an E2M1 code (its low four bits).
+__device__ __forceinline__ float e2m1_value(uint32_t code) {
+    const uint32_t e = code >> 1 & 3u, f = code & 1u;
+    const float v = e == 0 ? 0.5f * f : 0.5f * (2u + f) * (float)(1u << (e - 1));
+    return code & 8u ? -v : v;
+}
+// Rounded to odd: of the two neighbours of an inexact product the one whose last bit is set, which a second rounding, to two bits less or
+// fewer still, takes where it would have taken the product itself (Boldo and Melquiond, IEEE Trans. Comput. 57, 2008).
+__device__ __forceinline__ float product_to_odd(float a, float b) {
+    const float down = __fmul_rd(a, b), up = __fmul_ru(a, b);
+    return __float_as_uint(down) & 1u ? down : up;
 }
 // `n` values (at most 16) to element `p` on
 template <int TYPE>

@@ -784,3 +784,60 @@ def test_decode_rounds_once(module, dtype):
     if dtype != "f32":   # and rounding twice is something else here
         with np.errstate(all="ignore"):
             assert (plain.rounded_once(v.astype(np.float32), t) != plain.rounded_once(v, t)).sum() > 20
+
+
+# (exponent of A's scales, of B's, the codes of the block scales): the scales' product is subnormal, out of range below or above, or in
+# range with one of them far out
+ENDS = [(-110, -24, (0x28, 0x79)), (-60, -86, (0x28, 0x79)), (117, 13, (1, 2)), (126, -140, (0x28, 0x79)), (-110, 100, (0x28, 0x79)), (-149, 110, (0x40, 0x79)),
+        (127, 127, (0x28, 0x79)), (-149, -149, (0x28, 0x79)), (-70, -79, (0x70, 0x79))]
+
+
+def operand_at(rng, rows, k, per_row, exponent, s_range, zero_row):
+    codes = rng.integers(0, 16, (rows, k)).astype(np.uint8)
+    if zero_row is not None:
+        codes[zero_row] = 8 * rng.integers(0, 2, k)
+    s = rng.integers(*s_range, (rows, k // 16)).astype(np.uint8)
+    g = np.ldexp(rng.uniform(1, 1.9, rows if per_row else 1), exponent).astype(np.float32)
+    o = b2.Nvfp4Operand(torch.from_numpy(plain.pack(codes, -(-k // 32) * 16)).cuda(), torch.from_numpy(plain.tiled(s)).cuda(), torch.from_numpy(g).cuda(), rows, k)
+    return plain.values(codes, s, g), o
+
+
+def check_at_the_ends(got, want, terms, k, dtype):
+    got = plain.to_double(got)
+    bound = terms * (k * 2.0 ** -23 + 2.0 ** -22) + np.abs(want) * (2.0 ** -22 + plain.half_step(dtype)) + {torch.float32: 2.0 ** -148, torch.bfloat16: 2.0 ** -134}[dtype]
+    over = np.abs(want) + bound >= torch.finfo(dtype).max
+    assert not np.isnan(got).any()
+    assert (np.abs(got - want) <= bound)[~over].all()
+    sure = np.abs(want) - bound > 2.0 ** 128
+    assert (got[sure] == np.copysign(np.inf, want[sure])).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 70, 64), (60, 200, 4112), (140, 300, 272), (140, 301, 272), (1100, 2100, 64), (1100, 2101, 64)])
+@pytest.mark.parametrize("per_row", [(True, False), (True, True), (False, True)])
+def test_products_of_scales_at_the_ends_of_the_range(module, m, n, k, per_row):
+    """Results that FP32 has come out as they are, whatever the product of the two scales on top alone would be."""
+    rng = np.random.default_rng(m + n)
+    for ea, eb, s_range in ENDS:
+        a, oa = operand_at(rng, m, k, per_row[0], ea, s_range, 3)
+        b, ob = operand_at(rng, n, k, per_row[1], eb, s_range, None)
+        want, terms = a @ b.T, np.abs(a) @ np.abs(b).T
+        for dtype in (torch.float32, torch.bfloat16):
+            out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+            module.matmul(oa, ob, out)
+            check_at_the_ends(out, want, terms, k, dtype)
+            assert (out[3] == 0).all()
+    zero = b2.Nvfp4Operand(ob.bytes, ob.scales, torch.zeros_like(ob.scale), n, k)   # the scale of a tensor of zeros
+    out = torch.full((m, n), float("nan"), device="cuda")
+    module.matmul(oa, zero, out)
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("tokens,inputs", [(1, 256), (5, 1008), (12, 1008), (200, 256)])
+def test_small_activations_times_small_weights(module, tokens, inputs):
+    rng = np.random.default_rng(tokens)
+    x = torch.from_numpy((rng.standard_normal((tokens, inputs)) * 2.0 ** -101).astype(np.float32))
+    w, ow = operand_at(rng, 300, inputs, False, -22, (0x28, 0x79), None)
+    out = torch.empty(tokens, 300, device="cuda")
+    module.linear_forward(x.cuda(), ow, out, b2.Nvfp4LinearScratch(tokens, inputs, 300))
+    q = rounded(plain.to_double(x))
+    check_at_the_ends(out, q @ w.T, np.abs(q) @ np.abs(w).T, inputs, torch.float32)

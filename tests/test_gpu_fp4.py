@@ -841,3 +841,22 @@ def test_small_activations_times_small_weights(module, tokens, inputs):
     module.linear_forward(x.cuda(), ow, out, b2.Nvfp4LinearScratch(tokens, inputs, 300))
     q = rounded(plain.to_double(x))
     check_at_the_ends(out, q @ w.T, np.abs(q) @ np.abs(w).T, inputs, torch.float32)
+
+
+@pytest.mark.parametrize("rows,k", [(7, 40), (33, 100), (96, 128), (127, 250), (130, 70), (256, 64)])
+def test_quantisers_leave_rows_behind_the_last_one_alone(module, rows, k):
+    """Of a band of 128 rows a tensor owns the scales of its own; all 64-value tiles of these are written."""
+    x = torch.randn(rows, k, device="cuda")
+    for columns in (False, True):
+        o = b2.Nvfp4Operand.empty(rows, k, per_row=not columns)
+        o.scales.fill_(0x7f)
+        o.bytes.fill_(0x55)
+        if columns:
+            module.quantize_columns(x.T.contiguous(), o, torch.empty(b2.NVFP4_MAXIMA, device="cuda"))
+        else:
+            module.quantize_rows(x, o)
+        bands, chunks = -(-rows // 128), -(-o.k // 64)
+        all_rows, _ = plain.untiled(o.scales.cpu().numpy(), bands * 128, chunks * 4)
+        assert (all_rows[rows:] == 0x7f).all() and (all_rows[:rows, o.k // 16:] == 0).all()
+        assert (all_rows[:rows, :o.k // 16] < 0x7f).all() and (o.bytes[:, o.k // 2:] == 0x55).all()
+        check_operand(o, plain.to_double(x), whole=columns)

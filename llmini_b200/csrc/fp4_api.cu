@@ -145,14 +145,16 @@ int b2_nvfp4_linear_backward(const b2_nvfp4_linear_gradients *g, void *stream) {
     if (e == cudaSuccess && to_x) {
         e = along ? b2::launch_fp4_quantize_rows_and_maximum(g->grad, g->grad_rows, g->x, x_maxima, sms, s)
                   : launch_fp4_quantize_rows(g->grad, g->grad_rows, s);
-        if (e == cudaSuccess && g->grad_x.cols != 0) e = launch_fp4_matmul(g->grad_rows, g->weight_t, g->grad_x, nullptr, false, sms, s);
     }
-    if (e != cudaSuccess || !columns) return (int)e;
-    // the scales of grad's rows are scales of parts of it: with them its first pass is done
-    const b2::ColumnsTask tasks[2] = {{&g->grad, &g->grad_columns, to_x ? g->grad_rows.scale : nullptr, tokens},
-                                      {&g->x, &g->x_columns, x_maxima, along ? b2::fp4_maximum_parts(g->x, sms) : 0}};
-    e = launch_fp4_quantize_columns(tasks, 2, g->d_maxima, sms, s);
-    if (e == cudaSuccess) e = launch_fp4_matmul(g->grad_columns, g->x_columns, g->grad_weight, nullptr, g->accumulate != 0, sms, s);
+    if (e == cudaSuccess && columns) {
+        // the scales of grad's rows are scales of parts of it: with them its first pass is done
+        const b2::ColumnsTask tasks[2] = {{&g->grad, &g->grad_columns, to_x ? g->grad_rows.scale : nullptr, tokens},
+                                          {&g->x, &g->x_columns, x_maxima, along ? b2::fp4_maximum_parts(g->x, sms) : 0}};
+        e = launch_fp4_quantize_columns(tasks, 2, g->d_maxima, sms, s);
+    }
+    // grad and x have been read: grad_x may lie over either
+    if (e == cudaSuccess && to_x && g->grad_x.cols != 0) e = launch_fp4_matmul(g->grad_rows, g->weight_t, g->grad_x, nullptr, false, sms, s);
+    if (e == cudaSuccess && columns) e = launch_fp4_matmul(g->grad_columns, g->x_columns, g->grad_weight, nullptr, g->accumulate != 0, sms, s);
     return (int)e;
 }
 

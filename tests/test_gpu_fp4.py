@@ -860,3 +860,22 @@ def test_quantisers_leave_rows_behind_the_last_one_alone(module, rows, k):
         assert (all_rows[rows:] == 0x7f).all() and (all_rows[:rows, o.k // 16:] == 0).all()
         assert (all_rows[:rows, :o.k // 16] < 0x7f).all() and (o.bytes[:, o.k // 2:] == 0x55).all()
         check_operand(o, plain.to_double(x), whole=columns)
+
+
+@pytest.mark.parametrize("tokens,size", [(3, 96), (300, 320), (5000, 64)])
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f32", "bf16")])
+def test_gradients_over_their_inputs(module, tokens, size, types):
+    """grad_x in the place of x or of grad: both gradients are those of what lay there."""
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    x, grad = (torch.randn(tokens, size, device="cuda", generator=gen).to(TYPES[t]) for t in types)
+    wt = b2.Nvfp4Operand.empty(size, size)
+    module.quantize_rows(torch.randn(size, size, device="cuda", generator=gen), wt)
+    scratch = b2.Nvfp4LinearScratch(tokens, size, size, backward=True)
+    for place in (0, 1):
+        want = torch.empty_like((x, grad)[place]), torch.empty(size, size, device="cuda")
+        module.linear_backward(grad, x, wt, *want, scratch)
+        both = [x.clone(), grad.clone()]
+        got = both[place], torch.empty(size, size, device="cuda")
+        module.linear_backward(both[1], both[0], wt, *got, scratch)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert torch.equal(both[1 - place], (x, grad)[1 - place])

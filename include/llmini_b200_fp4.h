@@ -70,7 +70,7 @@ int b2_nvfp4_matmul(const b2_nvfp4_operand *a, const b2_nvfp4_operand *b, const 
 
 /* y = Q(x) W^T + bias: x [tokens][inputs] quantised by rows, W [outputs][inputs] as it is.  `scratch`: memory for Q(x), an operand of
  * tokens rows, scale_count = rows; a few values are quantised on the way and do not go there, so what it holds afterwards is not
- * defined. */
+ * defined.  y may lie over x; other buffers may not overlap. */
 int b2_nvfp4_linear_forward(const b2_matrix *x, const b2_nvfp4_operand *weight, const b2_matrix *y, const float *d_bias,
                             const b2_nvfp4_operand *scratch, void *stream);
 /* The gradients of that, straight through the rounding:

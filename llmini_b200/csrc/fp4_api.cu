@@ -45,6 +45,12 @@ bool rows_of(const b2_matrix &x, const b2_nvfp4_operand &o) {
 bool columns_of(const b2_matrix &x, const b2_nvfp4_operand &o) {
     return good(x) && good(o) && x.rows != 0 && o.rows == x.cols && o.cols == blocks_up(x.rows) && o.scale_count == 1;
 }
+// Whether two matrices may have a byte in common: whether their first and last bytes enclose one.
+bool may_overlap(const b2_matrix &a, const b2_matrix &b) {
+    auto first = [](const b2_matrix &m) { return reinterpret_cast<uintptr_t>(m.data); };
+    auto end = [&](const b2_matrix &m) { return first(m) + ((m.rows - 1) * m.ld + m.cols) * (m.type == B2_TYPE_F32 ? 4 : 2); };
+    return a.rows != 0 && b.rows != 0 && first(a) < end(b) && first(b) < end(a);
+}
 bool product_of(const b2_nvfp4_operand &a, const b2_nvfp4_operand &b, const b2_matrix &c) {
     return good(a) && good(b) && good(c) && a.cols == b.cols && c.rows == a.rows && c.cols == b.rows;
 }
@@ -110,8 +116,8 @@ int b2_nvfp4_linear_forward(const b2_matrix *x, const b2_nvfp4_operand *weight, 
     if (y->rows == 0 || y->cols == 0) return B2_SUCCESS;
     int sms = 0;
     cudaError_t e = sm_count(sms);
-    // a few values are quantised by every CTA of the product for itself; more, once
-    if (e == cudaSuccess && b2::fp4_linear_fused(x->rows, x->cols))
+    // a few values are quantised by every CTA of the product for itself; more, or what y lies over, once
+    if (e == cudaSuccess && b2::fp4_linear_fused(x->rows, x->cols) && !may_overlap(*x, *y))
         return (int)b2::launch_fp4_linear(*x, *weight, *y, d_bias, sms, as_stream(stream));
     if (e == cudaSuccess) e = launch_fp4_quantize_rows(*x, *scratch, as_stream(stream));
     if (e == cudaSuccess) e = launch_fp4_matmul(*scratch, *weight, *y, d_bias, false, sms, as_stream(stream));

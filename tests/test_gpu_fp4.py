@@ -879,3 +879,21 @@ def test_gradients_over_their_inputs(module, tokens, size, types):
         module.linear_backward(both[1], both[0], wt, *got, scratch)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert torch.equal(both[1 - place], (x, grad)[1 - place])
+
+
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1, 4800, 4800), (4, 1600, 1600), (3, 768, 2304), (1, 64, 200001), (5, 1600, 100000), (12, 1600, 1600), (300, 768, 512)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_over_its_input(module, tokens, inputs, outputs, dtype):
+    """y in the place of x, at its start or some rows on: what a call with a place of its own gives, time and again."""
+    rng = np.random.default_rng(tokens)
+    x = activations(rng, tokens, inputs, dtype).cuda()
+    _, w = operand(rng, outputs, inputs, False)
+    scratch, want = b2.Nvfp4LinearScratch(tokens, inputs, outputs), torch.empty(tokens, outputs, dtype=TYPES[dtype], device="cuda")
+    module.linear_forward(x, w, want, scratch)
+    for offset in (0, 7, (tokens - 1) * inputs):
+        memory = torch.empty(offset + tokens * max(inputs, outputs), dtype=TYPES[dtype], device="cuda")
+        for _ in range(10):
+            memory[:tokens * inputs].view_as(x).copy_(x)
+            y = memory[offset:offset + tokens * outputs].view(tokens, outputs)
+            module.linear_forward(memory[:tokens * inputs].view_as(x), w, y, scratch)
+            assert torch.equal(y, want)

@@ -59,7 +59,7 @@ int b2_nvfp4_quantize_rows(const b2_matrix *x, const b2_nvfp4_operand *out, void
 int b2_nvfp4_quantize_columns(const b2_matrix *x, const b2_nvfp4_operand *out, float *d_maxima, void *stream);
 /* The values of `in` in out's type, rounded once.  out: in.rows rows, in.cols - 15 .. in.cols columns.  scale_layout says how
  * in.scales is laid out: B2_SCALES_SM100, B2_SCALES_RAW ([rows][cols / 16]) or B2_SCALES_CSF (cols % 128 == 0); so the
- * optimizer's weights are read back too. */
+ * optimizer's weights are read back too.  CSF storage whose header describes fewer scales, or none, reads as NaN. */
 int b2_nvfp4_decode(const b2_nvfp4_operand *in, uint32_t scale_layout, const b2_matrix *out, void *stream);
 
 /* c[m][n] = sum_k a[m][k] b[n][k], + bias[n] (FP32, may be NULL), + c[m][n] where `accumulate` (FP32 c only).  a: M rows, b: N

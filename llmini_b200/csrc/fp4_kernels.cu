@@ -262,6 +262,13 @@ struct DecodeJob {
     uint64_t ld_bytes;
     uint32_t cols, access;
 };
+// Whether the header of CSF storage describes at least `groups` scales, and its records are of a size that there is (csf_load_scale goes
+// where it says).
+__device__ __forceinline__ bool csf_holds(const uint8_t *s, uint64_t groups) {
+    const uint32_t k = reinterpret_cast<const uint32_t *>(s)[0], rows = reinterpret_cast<const uint32_t *>(s)[1];
+    if (k == 0 || k % 128 != 0 || groups > (uint64_t)rows * (k / 16)) return false;
+    return rows == 1 ? s[8] == 255 : s[8] != 255 && (s[9] == 7 || s[9] == 8);
+}
 template <int TYPE>
 __device__ __forceinline__ void decode_rows(const DecodeJob &j) {
     const uint32_t row = blockIdx.x * (256u / j.threads_per_row) + threadIdx.x / j.threads_per_row;
@@ -272,7 +279,7 @@ __device__ __forceinline__ void decode_rows(const DecodeJob &j) {
     auto scale_of = [&](uint32_t blk) -> uint32_t {
         const uint64_t flat = (uint64_t)row * j.blocks + blk;
         return j.layout == B2_SCALES_SM100 ? j.scales[sm100_scale_offset(row, blk, tiles)]
-               : j.layout == B2_SCALES_RAW ? j.scales[flat] : csf_load_scale(j.scales, (uint32_t)flat);
+               : j.layout == B2_SCALES_RAW ? j.scales[flat] : csf_holds(j.scales, (uint64_t)j.rows * j.blocks) ? csf_load_scale(j.scales, (uint32_t)flat) : 0x7fu;
     };
     for (uint32_t blk = threadIdx.x % j.threads_per_row; blk < j.blocks; blk += j.threads_per_row) {
         const uint2 codes = codes_of(blk);

@@ -897,3 +897,31 @@ def test_linear_over_its_input(module, tokens, inputs, outputs, dtype):
             y = memory[offset:offset + tokens * outputs].view(tokens, outputs)
             module.linear_forward(memory[:tokens * inputs].view_as(x), w, y, scratch)
             assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 130])
+def test_decode_of_csf_storage_goes_by_its_header(module, rows):
+    """A header that is missing, of a smaller tensor or of no record size reads as NaN; the same scales under another shape are the same."""
+    k = 256
+    x = torch.randn(rows, k, device="cuda") * 0.02
+    raw = b2.Nvfp4Tensor.empty(rows, k, b2.SCALES_RAW)
+    b2.Nvfp4QuantModule().fp32_to_nvfp4_four_six(x, x.abs().max().reshape(1), raw.bytes, raw.scales, raw.global_scale, rows * k // 16, b2.SCALES_RAW)
+    want, out = torch.empty(rows, k, device="cuda"), torch.empty(rows, k, device="cuda")
+    module.decode(raw, want)
+    good = torch.from_numpy(b2.csf_encode_host(raw.scales.cpu().numpy(), rows, k)).cuda()
+
+    def read(scales, rows=rows, k=k):
+        out.zero_()
+        module.decode(b2.Nvfp4Tensor(raw.bytes, scales, raw.global_scale, rows, k, b2.SCALES_CSF), out.view(rows, k))
+        return out
+    assert torch.equal(read(good), want)
+    if rows > 1:
+        assert torch.equal(read(good, rows * 2, k // 2), want)
+    for at, values in ((0, [0, 0, 0, 0]), (0, [128, 0, 0, 0]), (0, [255, 255, 255, 255]), (0, [16, 1, 0, 0]), (4, [0, 0, 0, 0]), (4, [(rows - 1) % 256, 0, 0, 0]),
+                       (8, [255 if rows > 1 else 4]), (9, [6 if rows > 1 else 8])):
+        bad = good.clone()
+        bad[at:at + len(values)] = torch.tensor(values, dtype=torch.uint8, device="cuda")
+        if torch.equal(bad, good):
+            continue
+        assert torch.isnan(read(bad)).all(), (at, values)
+    assert torch.isnan(read(torch.zeros_like(good))).all()

@@ -91,7 +91,10 @@ class Nvfp4Tensor:
     @staticmethod
     def empty(rows: int, k: int, scale_layout: int = SCALES_CSF, device="cuda") -> "Nvfp4Tensor":
         n = rows * k
-        scales = zero_scales(rows, k, device) if scale_layout == SCALES_CSF else torch.zeros(n // 16, dtype=torch.uint8, device=device)
+        if scale_layout == SCALES_CSF:
+            scales = zero_scales(rows, k, device)
+        else:
+            scales = torch.zeros(sm100_scales_bytes(rows, k) if scale_layout == SCALES_SM100 else n // 16, dtype=torch.uint8, device=device)
         return Nvfp4Tensor(torch.zeros(n // 2, dtype=torch.uint8, device=device), scales,
                            torch.zeros(1, dtype=torch.float32, device=device), rows, k, scale_layout)
 

@@ -289,3 +289,15 @@ def test_plain_rounding():
     big = torch.finfo(torch.float16).max
     assert plain.rounded_once([big + 15.9, big + 16, -big - 16, 2.0 ** -25, 2.0 ** -24 * 1.5, -0.0], torch.float16).tolist() == [big, np.inf, -np.inf, 0, 2.0 ** -23, 0]
     assert plain.rounded_once([1 + 2.0 ** -8 + 2.0 ** -40], torch.bfloat16).tolist() == [1 + 2.0 ** -7]   # in two steps it would be 1
+
+
+@pytest.mark.parametrize("rows,k", [(1, 16), (33, 48), (128, 64), (130, 1600), (1000, 384)])
+def test_memory_of_a_tensor_in_every_scale_layout(rows, k):
+    """Nvfp4Tensor.empty has room for the scales in the layout that it is asked for."""
+    sizes = {b2.SCALES_RAW: rows * k // 16, b2.SCALES_SM100: -(-rows // 128) * -(-k // 64) * 512}
+    if k % 128 == 0:
+        sizes[b2.SCALES_CSF] = b2.csf_encoded_len(rows, k)
+    for layout, size in sizes.items():
+        t = b2.Nvfp4Tensor.empty(rows, k, layout, device="cpu")
+        assert (t.bytes.numel(), t.scales.numel(), t.scale_layout) == (rows * k // 2, size, layout)
+        assert layout == b2.SCALES_CSF or not t.scales.any()

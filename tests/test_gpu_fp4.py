@@ -925,3 +925,33 @@ def test_decode_of_csf_storage_goes_by_its_header(module, rows):
             continue
         assert torch.isnan(read(bad)).all(), (at, values)
     assert torch.isnan(read(torch.zeros_like(good))).all()
+
+
+@pytest.mark.parametrize("rows,k", [(1, 32), (33, 96), (128, 64), (130, 1600), (300, 160)])
+def test_operands_out_of_requantised_weights(module, rows, k):
+    """What the flat quantiser leaves, as the product's operand, by way of the converter or of memory that empty() gives."""
+    x = torch.randn(rows, k, device="cuda") * 0.02
+    raw = b2.Nvfp4Tensor.empty(rows, k, b2.SCALES_RAW)
+    b2.Nvfp4QuantModule().fp32_to_nvfp4_four_six(x, x.abs().max().reshape(1), raw.bytes, raw.scales, raw.global_scale, rows * k // 16, b2.SCALES_RAW)
+    tiled = b2.scales_to_sm100(raw.scales, b2.SCALES_RAW, rows, k)
+    t = b2.Nvfp4Tensor.empty(rows, k, b2.SCALES_SM100)
+    t.bytes.copy_(raw.bytes)
+    t.scales.copy_(tiled)
+    t.global_scale.copy_(raw.global_scale)
+    w = plain.values(plain.unpack(raw.bytes.cpu().numpy().reshape(rows, -1), k), raw.scales.cpu().numpy().reshape(rows, -1), raw.global_scale.item())
+    a = torch.randn(50, k, device="cuda")
+    for tensor in (b2.Nvfp4Tensor(raw.bytes, tiled, raw.global_scale, rows, k, b2.SCALES_SM100), t):
+        o = b2.Nvfp4Operand.from_tensor(tensor)
+        assert o.bytes.data_ptr() == tensor.bytes.data_ptr() and (o.rows, o.k) == (rows, k)
+        out = torch.empty(50, rows, device="cuda")
+        module.linear_forward(a, o, out, b2.Nvfp4LinearScratch(50, k, rows))
+        within(out, rounded(plain.to_double(a)), w, torch.float32)
+        back = torch.empty(rows, k, device="cuda")
+        module.decode(tensor, back)
+        np.testing.assert_array_equal(plain.to_double(back), plain.rounded_once(w, torch.float32))
+    for bad in (raw, b2.Nvfp4Tensor(raw.bytes, tiled[:-1], raw.global_scale, rows, k, b2.SCALES_SM100)):
+        with pytest.raises(ValueError):
+            b2.Nvfp4Operand.from_tensor(bad)
+    if rows > 1:
+        with pytest.raises(ValueError):
+            b2.Nvfp4Operand.from_tensor(b2.Nvfp4Tensor.empty(rows, 48, b2.SCALES_SM100))

@@ -955,3 +955,61 @@ def test_operands_out_of_requantised_weights(module, rows, k):
     if rows > 1:
         with pytest.raises(ValueError):
             b2.Nvfp4Operand.from_tensor(b2.Nvfp4Tensor.empty(rows, 48, b2.SCALES_SM100))
+
+
+# few rows over more tiles of columns than there are SMs (pipelines shorter than K, several CTAs an SM), over a long K, and the 33 .. 64
+# rows that take the few rows' way where K is long
+FEW_ROWS = [(1, 50257, 1600), (8, 50257, 1600), (32, 50257, 1600), (33, 1600, 6400), (40, 1600, 6400), (64, 1600, 6400), (64, 48, 4112), (3, 64, 33008),
+            (64, 20000, 4096), (17, 129, 70000)]
+
+
+@pytest.mark.parametrize("m,n,k", FEW_ROWS)
+def test_matmul_of_few_rows(module, m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    a, oa = operand(rng, m, k, True)
+    b, ob = operand(rng, n, k, False, 16)
+    want, bound = a @ b.T, None
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+        module.matmul(oa, ob, out)
+        assert module.status() == 0
+        bound = product_bound(a, b, want, dtype)
+        assert (np.abs(plain.to_double(out) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1, 1600, 50257), (8, 1000, 20000), (1, 1001, 50257), (1, 7, 33), (3, 1001, 300), (8, 1024, 19000), (2, 4095, 64), (8, 33, 129)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("offset,gap", [(0, 0), (1, 0), (8, 8), (3, 5)])
+def test_linear_of_few_rows(module, tokens, inputs, outputs, dtype, offset, gap):
+    """Rows quantised inside the product: of any length, with gaps, on any boundary; what is around them is not read into them."""
+    rng = np.random.default_rng(tokens + outputs + offset)
+    x = activations(rng, tokens, inputs, dtype) / 64
+    memory = torch.full((offset + tokens * (inputs + gap),), float("nan"), dtype=x.dtype, device="cuda")
+    view = memory[offset:].view(tokens, inputs + gap)[:, :inputs]
+    view.copy_(x)
+    k = -(-inputs // 16) * 16
+    w, ow = operand(rng, outputs, k, False)
+    out = torch.empty(tokens, outputs, device="cuda")
+    module.linear_forward(view, ow, out, b2.Nvfp4LinearScratch(tokens, inputs, outputs))
+    q = np.zeros((tokens, k))
+    q[:, :inputs] = rounded(plain.to_double(x))
+    within(out, q, w, torch.float32)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 6400), (5, 20000, 1600), (64, 130, 6400), (24, 1600, 6400), (3, 64, 33008), (300, 500, 6400), (140, 301, 16400), (1100, 2100, 1616),
+                                   (1100, 2101, 4000)])
+def test_matmul_of_exact_sums(module, m, n, k):
+    """Products that are multiples of 1/4 and add up to less than 2^22: FP32 has every sum, in any order, so nothing may be missing."""
+    rng = np.random.default_rng(k + m)
+    s_range = (1,) if k > 6400 else (1, 2, 4)   # 6 6 s s 6400 < 2^22
+    sides = []
+    for rows in (m, n):
+        codes = rng.integers(0, 16, (rows, k)).astype(np.uint8)
+        s = rng.choice([0x38 + 8 * int(np.log2(v)) for v in s_range], (rows, k // 16)).astype(np.uint8)
+        sides.append((plain.values(codes, s, [1.0]), b2.Nvfp4Operand(torch.from_numpy(plain.pack(codes, -(-k // 32) * 16)).cuda(),
+                                                                     torch.from_numpy(plain.tiled(s)).cuda(), torch.ones(1, device="cuda"), rows, k)))
+    (a, oa), (b, ob) = sides
+    assert (np.abs(a).max() * np.abs(b).max()) * k < 2 ** 22
+    out = torch.empty(m, n, device="cuda")
+    module.matmul(oa, ob, out)
+    np.testing.assert_array_equal(plain.to_double(out), a @ b.T)

@@ -125,7 +125,7 @@ int b2_nvfp4_cache_write(const b2_nvfp4_cache *caches, const b2_vectors *tokens,
                          uint32_t token_count, void *stream);
 /* Reads sequence b's tokens 0 .. d_lengths[b] (clamped to [0, min(max_tokens, table_width * page_size)]) of each cache into
  * out: token t lies in page d_table[b][t / page_size].  A page outside [0, pages) reads as NaN.  What lies behind a sequence's
- * length in out is left as it is. */
+ * length in out is left as it is.  Vectors of out may not overlap. */
 int b2_nvfp4_cache_read(const b2_nvfp4_cache *caches, const b2_vectors *out, uint32_t count, const int32_t *d_table,
                         uint32_t table_width, const int32_t *d_lengths, uint32_t sequences, uint32_t max_tokens, void *stream);
 

@@ -114,6 +114,16 @@ def _matrix(t: torch.Tensor, device: int) -> bytes:
         _refuse("rows and columns are 32-bit numbers")
 
 
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether values of a tensor lie in one place: whether a dimension's step is shorter than what the smaller steps reach over."""
+    reach = 1
+    for step, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n != 1):
+        if step < reach and t.numel():
+            return True
+        reach += step * (n - 1)
+    return False
+
+
 def _floats(t: torch.Tensor, count: int, what: str, device: int) -> int:
     if t.dtype != torch.float32 or t.numel() < count or not t.is_contiguous():
         _refuse(f"{what}: {count} contiguous FP32 values are wanted")
@@ -341,11 +351,14 @@ class Nvfp4LinearModule:
             t, shape, stride = tensors[i], tensors[i].shape, tensors[i].stride()
             if shape[-2:] != cache.sizes[i] or stride[-1] != 1:
                 _refuse("vectors of the cache's heads and size, their values side by side")
-            if dims == 4 and any(n > 1 and s == 0 for n, s in zip(shape, stride)):
+            if dims == 4 and not t.is_contiguous() and _overlaps(t):
                 _refuse("vectors that are written lie apart")
             if i and (t.dtype != first.dtype or shape[:-2] != first.shape[:-2]):
                 _refuse("keys and values: tensors of one type and length")
-            v += _vectors_bytes(_here(t, d), stride[0] if dims == 4 else 0, stride[-3], stride[-2], kind, 0)
+            at = _here(t, d)
+            if dims == 4 and i and at == first.data_ptr() and t.numel():
+                _refuse("keys and values go to places of their own")
+            v += _vectors_bytes(at, stride[0] if dims == 4 else 0, stride[-3], stride[-2], kind, 0)
         return v, n, first.shape
 
     def cache_write(self, cache: Nvfp4PagedCache, slots: torch.Tensor, key: torch.Tensor, value: torch.Tensor | None = None) -> None:

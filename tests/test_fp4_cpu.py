@@ -301,3 +301,19 @@ def test_memory_of_a_tensor_in_every_scale_layout(rows, k):
         t = b2.Nvfp4Tensor.empty(rows, k, layout, device="cpu")
         assert (t.bytes.numel(), t.scales.numel(), t.scale_layout) == (rows * k // 2, size, layout)
         assert layout == b2.SCALES_CSF or not t.scales.any()
+
+
+def test_results_of_a_cache_lie_apart():
+    """Vectors that are read into may be in any order and at any distance, but not over one another."""
+    n = 4096
+    memory = torch.zeros(n).as_subclass(OnDevice)
+    shapes = [((2, 3, 4, 16), s) for s in ((192, 64, 16, 1), (192, 16, 48, 1), (64, 128, 16, 1), (16, 32, 96, 1), (500, 100, 17, 1), (1024, 64, 16, 1))]
+    shapes += [((1, 3, 4, 16), (0, 64, 16, 1)), ((2, 1, 1, 16), (16, 0, 0, 1)), ((1, 1, 1, 16), (5, 5, 5, 1)), ((0, 3, 4, 16), (0, 0, 0, 1))]
+    for shape, stride in shapes:
+        assert not fp4._overlaps(memory.as_strided(shape, stride)), stride
+    for shape, stride in (((2, 3, 4, 16), (191, 64, 16, 1)), ((2, 3, 4, 16), (192, 63, 16, 1)), ((2, 3, 4, 16), (192, 64, 15, 1)), ((2, 3, 4, 16), (64, 64, 16, 1)),
+                          ((2, 3, 4, 16), (0, 64, 16, 1)), ((5, 1, 1, 16), (8, 0, 0, 1)), ((2, 3, 4, 16), (16, 64, 16, 1))):
+        t = memory.as_strided(shape, stride)
+        assert fp4._overlaps(t), stride
+        places = torch.arange(n).as_strided(shape, stride).flatten()
+        assert len(places.unique()) < len(places)

@@ -1013,3 +1013,16 @@ def test_matmul_of_exact_sums(module, m, n, k):
     out = torch.empty(m, n, device="cuda")
     module.matmul(oa, ob, out)
     np.testing.assert_array_equal(plain.to_double(out), a @ b.T)
+
+
+def test_a_cache_is_not_read_into_the_same_place_twice(module):
+    cache = b2.Nvfp4PagedCache.empty(4, 8, 2, 32)
+    table, lengths = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    good, memory = torch.zeros(3, 8, 2, 32, device="cuda"), torch.zeros(4096, device="cuda")
+    for strides in ((256, 64, 32, 1), (511, 32, 256, 1)):
+        for bad in (memory.as_strided((3, 8, 2, 32), strides), good):
+            with pytest.raises(ValueError):
+                module.cache_read(cache, table, lengths, bad, good)
+    both = torch.zeros(3, 8, 2, 2, 32, device="cuda")
+    module.cache_read(cache, table, lengths, both[:, :, 0], both[:, :, 1])
+    module.cache_read(cache, table, lengths, memory.as_strided((3, 8, 2, 32), (512, 32, 256, 1)), good)   # head by head

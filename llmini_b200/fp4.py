@@ -293,7 +293,7 @@ class Nvfp4LinearModule:
             need = _up(t.rows, 128) * _up(t.k // 16, 4) if layout == SCALES_SM100 else t.rows * t.k // 16 if layout == SCALES_RAW else _csf_bytes(t.rows, t.k)
             if t.bytes.numel() < t.rows * t.k // 2 or t.scales.numel() < need or not (t.bytes.is_contiguous() and t.scales.is_contiguous()):
                 _refuse("an Nvfp4Tensor with too little memory for its rows and k, or with gaps in it")
-            c = C.byref(Operand(_here(t.bytes, d), _here(t.scales, d), _here(t.global_scale, d), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
+            c = C.byref(Operand(_here(t.bytes, d), _here(t.scales, d), _floats(t.global_scale, 1, "global_scale", d), _up(t.k // 2, 16), t.rows, t.k, 1, 0))
         else:
             c, layout = _operand(operand, d), SCALES_SM100
         check(self._lib.b2_nvfp4_decode(c, layout, _matrix(out, d), _stream_of(d)), "nvfp4_decode")

@@ -1026,3 +1026,12 @@ def test_a_cache_is_not_read_into_the_same_place_twice(module):
     both = torch.zeros(3, 8, 2, 2, 32, device="cuda")
     module.cache_read(cache, table, lengths, both[:, :, 0], both[:, :, 1])
     module.cache_read(cache, table, lengths, memory.as_strided((3, 8, 2, 32), (512, 32, 256, 1)), good)   # head by head
+
+
+def test_decode_refuses_another_scale_type(module):
+    out = torch.empty(4, 32, device="cuda")
+    for bad in (torch.ones(1, dtype=torch.float64, device="cuda"), torch.ones(1, dtype=torch.bfloat16, device="cuda"), torch.ones(0, device="cuda"), torch.ones(1)):
+        t = b2.Nvfp4Tensor.empty(4, 32, b2.SCALES_RAW)
+        t.global_scale = bad
+        with pytest.raises(ValueError):
+            module.decode(t, out)

@@ -28,7 +28,7 @@ namespace {
 
 constexpr uint32_t kStageK = 256;       // values of K in a pipeline stage
 constexpr uint32_t kScaleTile = 512;    // bytes: 128 rows x 64 values of K
-constexpr uint32_t kSlabs = 1, kSlabBytes = kSlabs * 32 * 128;   // an epilogue warp's: 32 rows x 128 bytes of c each
+constexpr uint32_t kSlabBytes = 32 * 128;   // an epilogue warp's: 32 rows x 128 bytes of c
 constexpr uint32_t kScaleBand = kStageK / 64 * kScaleTile;   // a stage's scales of 128 rows
 
 // Set when a bounded wait ran out (b2_nvfp4_status).
@@ -394,9 +394,8 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
         // shared memory (32 rows x 128 bytes) to bulk stores of whole lines.
         const uint32_t q = warp & 3, half = (warp - C::kEpiWarp0) >> 2;
         const uint32_t tempty_leader = PAIR ? map_to_cta(tempty_bar(0), 0) : tempty_bar(0);
-        uint8_t *slabs = smem + C::kStages * C::kStageBytes + C::kControl + (warp - C::kEpiWarp0) * kSlabBytes;
+        uint8_t *slab_bytes = smem + C::kStages * C::kStageBytes + C::kControl + (warp - C::kEpiWarp0) * kSlabBytes;
         float *strip = reinterpret_cast<float *>(smem + C::kStages * C::kStageBytes + C::kControl + C::kEpiWarps * kSlabBytes + (warp - C::kEpiWarp0) * C::kStrip);
-        uint32_t turn = 0;
         const float sb = epi.b_rows ? 1.0f : *epi.scale_b;
         uint32_t it = 0;
         for (uint32_t t = first; t < tiles; t += stride, ++it) {
@@ -465,7 +464,7 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                 }
                 const bool f32 = epi.type == B2_TYPE_F32;
                 if (!BULK) {
-                    const uint32_t slab = smem_u32(slabs);
+                    const uint32_t slab = smem_u32(slab_bytes);
                     const bool whole = epi.classes != 0 && row0 + 32 <= epi.M && col0 + (unit == 0 ? 72 : 64) <= epi.N;
                     const bool last = (unit + 1) * 64 == BN || col0 + 128 > epi.N;   // of the tile's whole units
                     if (lane < 8) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");   // the last stores have read the slab
@@ -477,7 +476,7 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                             if (col >= epi.N) continue;
                             float v[32];
                             finish_columns(epi, col, min(32u, epi.N - col), r[part], s, epi.bias ? strip + 32 * part : nullptr, v);
-                            store_through(epi, row0, col, v, reinterpret_cast<float *>(slabs));
+                            store_through(epi, row0, col, v, reinterpret_cast<float *>(slab_bytes));
                         }
                         continue;
                     }
@@ -564,14 +563,14 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                     finish_columns(epi, col, min(32u, epi.N - col), r[part], s, epi.bias ? strip + 32 * part : nullptr, v);
                     if (epi.accumulate && col + 32 > epi.N) {
                         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        store_through(epi, row0, col, v, reinterpret_cast<float *>(slabs));
+                        store_through(epi, row0, col, v, reinterpret_cast<float *>(slab_bytes));
                         continue;
                     }
                     if (f32 || part == 0) {   // the store that read this slab last is through with it
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlabs - 1) : "memory");
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         __syncwarp();
                     }
-                    const uint32_t slab = smem_u32(slabs) + turn * 4096, slab_row = slab + lane * 128;
+                    const uint32_t slab = smem_u32(slab_bytes), slab_row = slab + lane * 128;
                     if (f32) {
                         if (epi.accumulate && row < epi.M) add_old(epi, row, col, v);
 #pragma unroll
@@ -591,7 +590,6 @@ k_fp4_gemm(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CU
                     fence_async_smem();
                     __syncwarp();
                     if (lane == 0) tma_store_2d(reinterpret_cast<uint64_t>(&map_c), slab, (int)(f32 ? col : col0), (int)row0);
-                    turn = turn + 1 == kSlabs ? 0 : turn + 1;
                 }
             }
         }

@@ -77,8 +77,8 @@ int b2_nvfp4_linear_forward(const b2_matrix *x, const b2_nvfp4_operand *weight, 
  *   grad_x = Q(grad) W          Q by rows; weight_t is W^T [inputs][outputs], quantised along the outputs
  *   grad_weight = Q(grad^T) Q(x^T)^T   both quantised along the tokens, one scale a tensor; FP32, added to what is there where
  *                               `accumulate`
- * grad_x.data or grad_weight.data may be NULL: that gradient is left out.  grad and x have been read before a result is written, so
- * grad_x may lie over either; other buffers may not overlap.  Scratch: grad_rows as `scratch` above for grad,
+ * grad_x.data or grad_weight.data may be NULL: that gradient is left out.  grad_x may lie over grad or over x; other
+ * buffers may not overlap.  Scratch: grad_rows as `scratch` above for grad,
  * grad_columns [outputs][tokens] and x_columns [inputs][tokens] as of b2_nvfp4_quantize_columns, d_maxima. */
 typedef struct b2_nvfp4_linear_gradients {
     b2_matrix grad;            /* [tokens][outputs] */

@@ -148,9 +148,14 @@ int b2_nvfp4_linear_backward(const b2_nvfp4_linear_gradients *g, void *stream) {
     // 64 x 1024 -> 1024 15.0 -> 13.3; with 8192 rows 85.9 -> 86.8
     const bool along = to_x && columns && g->x.type == g->grad.type && tokens <= b2::kFewTops;
     float *x_maxima = along ? g->d_maxima + B2_NVFP4_MAXIMA : nullptr;
+    // grad_x comes last of all where it lies over what the columns are still to be read from.  (Always last, 777 x 1600 -> 1600 on new inputs
+    // takes 26.5 us instead of 25.7, on the same ones again 23.7 instead of 24.4.)
+    const bool last = columns && (may_overlap(g->grad_x, g->grad) || may_overlap(g->grad_x, g->x));
+    auto product_x = [&]() { return to_x && g->grad_x.cols != 0 ? launch_fp4_matmul(g->grad_rows, g->weight_t, g->grad_x, nullptr, false, sms, s) : cudaSuccess; };
     if (e == cudaSuccess && to_x) {
         e = along ? b2::launch_fp4_quantize_rows_and_maximum(g->grad, g->grad_rows, g->x, x_maxima, sms, s)
                   : launch_fp4_quantize_rows(g->grad, g->grad_rows, s);
+        if (e == cudaSuccess && !last) e = product_x();
     }
     if (e == cudaSuccess && columns) {
         // the scales of grad's rows are scales of parts of it: with them its first pass is done
@@ -158,8 +163,7 @@ int b2_nvfp4_linear_backward(const b2_nvfp4_linear_gradients *g, void *stream) {
                                           {&g->x, &g->x_columns, x_maxima, along ? b2::fp4_maximum_parts(g->x, sms) : 0}};
         e = launch_fp4_quantize_columns(tasks, 2, g->d_maxima, sms, s);
     }
-    // grad and x have been read: grad_x may lie over either
-    if (e == cudaSuccess && to_x && g->grad_x.cols != 0) e = launch_fp4_matmul(g->grad_rows, g->weight_t, g->grad_x, nullptr, false, sms, s);
+    if (e == cudaSuccess && last) e = product_x();
     if (e == cudaSuccess && columns) e = launch_fp4_matmul(g->grad_columns, g->x_columns, g->grad_weight, nullptr, g->accumulate != 0, sms, s);
     return (int)e;
 }

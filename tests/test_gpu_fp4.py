@@ -1035,3 +1035,29 @@ def test_decode_refuses_another_scale_type(module):
         t.global_scale = bad
         with pytest.raises(ValueError):
             module.decode(t, out)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 300, 64), (140, 300, 272), (140, 301, 272), (1100, 2101, 64)])
+def test_rows_of_zeros_beside_small_weights(module, m, n, k):
+    """The scale of a row of zeros is the least that there is, and its product with a small weight's is subnormal: the row stays zero and the
+    others are what they are without it, bit for bit, with tiny rows among them too."""
+    rng = np.random.default_rng(m)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    w, ow = operand_at(rng, n, k, False, -20, (0x28, 0x79), None)
+    bias = torch.randn(n, device="cuda")
+    outs = []
+    for zeros in (False, True):
+        x[1::3] *= not zeros
+        x[5] *= np.float32(2.0 ** -102) if zeros else 1
+        for dtype in (torch.float32, torch.bfloat16):
+            out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+            module.linear_forward(torch.from_numpy(x).cuda(), ow, out, b2.Nvfp4LinearScratch(m, k, n), bias=bias)
+            outs.append(out)
+    kept = np.setdiff1d(np.arange(m), np.r_[1:m:3, 5])
+    for whole, some in zip(outs[:2], outs[2:]):
+        assert torch.equal(whole[kept], some[kept])
+        assert (some[1::3] == bias.to(some.dtype)).all()
+    q = rounded(x.astype(np.float64))
+    out = torch.empty(m, n, device="cuda")
+    module.linear_forward(torch.from_numpy(x).cuda(), ow, out, b2.Nvfp4LinearScratch(m, k, n))
+    check_at_the_ends(out, q @ w.T, np.abs(q) @ np.abs(w).T, k, torch.float32)

@@ -1061,3 +1061,20 @@ def test_rows_of_zeros_beside_small_weights(module, m, n, k):
     out = torch.empty(m, n, device="cuda")
     module.linear_forward(torch.from_numpy(x).cuda(), ow, out, b2.Nvfp4LinearScratch(m, k, n))
     check_at_the_ends(out, q @ w.T, np.abs(q) @ np.abs(w).T, k, torch.float32)
+
+
+@pytest.mark.parametrize("tokens,inputs", [(2, 160), (8, 1008), (20, 6400), (60, 4160), (300, 160)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_that_are_not_finite_stay_apart(module, tokens, inputs, dtype):
+    rng = np.random.default_rng(tokens)
+    x = activations(rng, tokens, inputs, dtype) / 64
+    good = x.clone()
+    x[1, 3], x[-1, inputs - 1] = float("inf"), float("nan")
+    w, ow = operand(rng, 200, inputs, False)
+    out = torch.zeros(tokens, 200, device="cuda")
+    module.linear_forward(x.cuda(), ow, out, b2.Nvfp4LinearScratch(tokens, inputs, 200))
+    bad = np.isin(np.arange(tokens), [1, tokens - 1])
+    got, q = plain.to_double(out), rounded(plain.to_double(good))
+    want = q @ w.T
+    assert np.isnan(got[bad]).all()
+    assert (np.abs(got - want) <= product_bound(q, w, want, torch.float32))[~bad].all()

@@ -1082,19 +1082,19 @@ cudaError_t launch_fp4_matmul(const b2_nvfp4_operand &a, const b2_nvfp4_operand 
         if (k == 3) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
     }
 #endif
-    // Few rows: 24 x 1600 -> 50304 takes 8.5 us, in tiles 17.6; 24 x 6400 -> 1600, eight CTAs sharing K, 5.8 and 11.0; 16 x 768 ->
-    // 2304 is even (4.1, 3.8).  From 33 rows on only a long K pays: 64 x 6400 -> 1600 7.2 and 11.1, 64 x 1600 -> 4800 7.6 and 5.5.
+    // Few rows: 24 x 1600 -> 50304 takes 8.7 us, in tiles 15.0; 24 x 6400 -> 1600, eight CTAs sharing K, 5.8 and 10.8; 16 x 768 ->
+    // 2304 is about even (4.3, 3.8).  From 33 rows on only a long K pays: 64 x 6400 -> 1600 7.2 and 11.1, 64 x 1600 -> 4800 7.6 and 5.5.
     if (a.rows <= kFewRows / 2 || (a.rows <= kFewRows && a.cols >= 4096)) return few_impl<-1>(&a, nullptr, b, epi, sm_count, s);
-    // Tiles of one CTA while every one of them has an SM to itself (777 x 1600 -> 1600 6.0 us, in pairs 7.1; 1000 x 768 -> 2304 4.6
-    // and 5.8), else pairs, which take in half as much for an operation (200 x 1600 -> 50304 20.7 and 14.5; 2000 x 6400 -> 1600 20.4
-    // and 13.0; 512 x 1600 -> 4800, 152 tiles, 8.0 and 7.2).
+    // Tiles of one CTA while every one of them has an SM to itself (777 x 1600 -> 1600 6.0 us, in pairs 7.0; 1000 x 768 -> 2304 4.7
+    // and 5.8), else pairs, which take in half as much for an operation (200 x 1600 -> 50304 20.9 and 14.8; 2000 x 6400 -> 1600 20.8
+    // and 13.3; 512 x 1600 -> 4800, 152 tiles, 8.0 and 7.2).
     const uint64_t tiles = (uint64_t)((a.rows + 127) / 128) * ((b.rows + 127) / 128);
     if (tiles > (uint64_t)sm_count) return gemm_impl<true, 256>(a, b, c, epi, sm_count, s);
     return gemm_impl<false, 128>(a, b, c, epi, sm_count, s);
 }
 
-// Quantised on the way and as a launch of its own: 1 x 1600 -> 4800 5.3 us and 7.0, 4 x 1600 -> 4800 6.5 and 7.3, 8 x 1600 -> 4800 8.1
-// and 7.6, 1 x 6400 -> 1600 6.6 and 7.5, 2 x 6400 -> 1600 7.6 and 7.7.
+// Quantised on the way and as a launch of its own: 1 x 1600 -> 4800 5.4 us and 6.6, 4 x 1600 -> 4800 6.4 and 6.8, 8 x 1600 -> 4800 7.6
+// and 7.0, 1 x 6400 -> 1600 6.8 and 7.2, 2 x 6400 -> 1600 7.8 and 7.4.
 bool fp4_linear_fused(uint32_t rows, uint32_t cols) { return rows <= kFusedRows && (uint64_t)rows * cols <= 8192; }
 
 cudaError_t launch_fp4_linear(const b2_matrix &x, const b2_nvfp4_operand &b, const b2_matrix &c, const float *bias, int sm_count, cudaStream_t s) {

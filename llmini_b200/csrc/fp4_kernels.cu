@@ -3,9 +3,9 @@
 // long, so they issue in 60 to 70 % of the cycles.
 //
 // The work is 16 values a thread, a whole block, so its maximum needs no exchange.  Measured, BF16, inputs partly in L2 as a layer's
-// are; in brackets the bytes at the rate of a copy: 16384 x 1600 by rows 12.7 us (10.3); by columns 19.4, 8 of them the maximum
-// (10.3, 18.3 with x read twice); decode by rows 13.1, of 1600 x 16384 10.5 (10.3); 32768 tokens of two 16 x 64 vectors written to the
-// cache 34.5 us (26.5), as many read back 33 (26.5).
+// are; in brackets the bytes at the rate of a copy: 16384 x 1600 by rows 12.8 us (10.3); by columns 19.4, 8 of them the maximum
+// (10.3, 18.3 with x read twice); decode by rows 14.3, of 1600 x 16384 10.6 (10.3); 32768 tokens of two 16 x 64 vectors written to the
+// cache 35 us (26.5), as many read back 31 (26.5).
 #include <algorithm>
 
 #include "common.cuh"
